@@ -1,0 +1,233 @@
+// The paged key/value cache and rotary tables: what a call has to satisfy, where a row lies, and how a sequence is split over
+// workgroups. Plain C++ (no HIP), so that all of it is checked without a GPU; the kernels use the same functions.
+#pragma once
+#include <cmath>
+#include <cstddef>
+#include <cstdint>
+
+#include "elmh.h"
+
+#ifdef __HIPCC__
+#define ELM_HD __host__ __device__ inline
+#else
+#define ELM_HD inline
+#endif
+
+namespace elmh {
+
+// ---------------------------------------------------------------- layout
+
+constexpr int kPageStep = 16;   // pages hold a multiple of this many positions: one matrix-instruction tile of tokens
+constexpr int kSplitUnit = 32;  // tokens a wave takes at a time; a sequence is split at multiples of it
+
+ELM_HD bool kv_quantized(int dtype) { return dtype == ELMH_Q8 || dtype == ELMH_Q4; }
+// f32 scales per row
+ELM_HD int kv_groups(int dtype, int head_dim) { return dtype == ELMH_Q8 ? 1 : dtype == ELMH_Q4 ? head_dim / 32 : 0; }
+// bytes of one row's values
+ELM_HD int kv_row_bytes(int dtype, int head_dim) {
+  return dtype == ELMH_F32 ? 4 * head_dim : dtype == ELMH_Q8 ? head_dim : dtype == ELMH_Q4 ? head_dim / 2 : 2 * head_dim;
+}
+// Rows [page][kv head][slot]: the index of a row, and of its first scale ([page][kv head][group][slot], groups page_size apart)
+ELM_HD int64_t kv_row(int64_t page, int head, int slot, int n_kv, int page_size) {
+  return (page * n_kv + head) * page_size + slot;
+}
+ELM_HD int64_t kv_scale(int64_t page, int head, int slot, int n_kv, int page_size, int groups) {
+  return (page * n_kv + head) * groups * page_size + slot;
+}
+// The byte of a q4 row that holds value d (even d in the low nibble). Keys: [c][j][b], values 32 j + 8 c + 2 b, so that the
+// eight values a lane multiplies of each group are one word and its words of all groups are contiguous. Value rows: [i][j],
+// values 32 j + 2 i, so that sixteen lanes hold one group's values in the same byte.
+ELM_HD int q4_key_byte(int d, int head_dim) { return (d % 32 / 8) * (head_dim / 8) + d / 32 * 4 + d % 8 / 2; }
+ELM_HD int q4_value_byte(int d, int head_dim) { return d % 32 / 2 * (head_dim / 32) + d / 32; }
+
+// The page of position pos in a sequence's row of the table, or -1: no such entry, or no such page
+ELM_HD int64_t kv_page_of(const int32_t* table_row, int max_pages, int64_t n_pages, int pos, int page_size) {
+  const int i = pos / page_size;
+  if (pos < 0 || i >= max_pages) return -1;
+  const int64_t p = table_row[i];
+  return p >= 0 && p < n_pages ? p : -1;
+}
+
+// ---------------------------------------------------------------- the split of a sequence
+
+// Units of kSplitUnit tokens per part when `units` are split over at most `parts`, each of at least `least`
+ELM_HD int split_size(int units, int parts, int least) {
+  const int per = (units + parts - 1) / parts;
+  return per > least ? per : least;
+}
+ELM_HD int split_parts(int units, int per) { return (units + per - 1) / per; }
+
+// ---------------------------------------------------------------- what a call has to satisfy
+
+struct PagedFault {
+  int code = ELMH_OK;
+  const char* what = nullptr;
+};
+
+inline bool kv_head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 192 || hd == 256; }
+
+inline PagedFault check_kv_shape(int dtype, int n_kv, int head_dim, int page_size) {
+  if (dtype != ELMH_F32 && dtype != ELMH_F16 && dtype != ELMH_BF16 && !kv_quantized(dtype))
+    return {ELMH_ERR_UNSUPPORTED, "cache type: f32, f16, bf16, q8 and q4 are held"};
+  if (n_kv < 1 || n_kv > 1024) return {ELMH_ERR_ARG, "kv heads outside 1 .. 1024"};
+  if (!kv_head_dim_ok(head_dim)) return {ELMH_ERR_UNSUPPORTED, "head_dim: 32, 64, 96, 128, 192 and 256 are held"};
+  if (page_size < kPageStep || page_size % kPageStep || page_size > 4096)
+    return {ELMH_ERR_ARG, "page_size: a multiple of 16 up to 4096"};
+  return {};
+}
+
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+inline PagedFault check_kv_pages(const elmh_kv_pages* p) {
+  if (!p) return {ELMH_ERR_ARG, "null pages"};
+  const PagedFault f = check_kv_shape(p->dtype, p->n_kv, p->head_dim, p->page_size);
+  if (f.code) return f;
+  if (p->n_pages < 1 || p->n_pages > INT32_MAX) return {ELMH_ERR_ARG, "n_pages outside 1 .. 2^31 - 1"};
+  if (!p->k || !p->v) return {ELMH_ERR_ARG, "null key or value pool"};
+  if (!aligned16(p->k) || !aligned16(p->v)) return {ELMH_ERR_ARG, "pools start on 16 bytes"};
+  if (kv_quantized(p->dtype)) {
+    if (!p->k_scale || !p->v_scale) return {ELMH_ERR_ARG, "null scales of a quantized cache"};
+    if (!aligned16(p->k_scale) || !aligned16(p->v_scale)) return {ELMH_ERR_ARG, "scales start on 16 bytes"};
+  }
+  return {};
+}
+
+inline PagedFault check_rope(const elmh_rope* r, int head_dim) {
+  if (!r) return {};
+  if (!r->cos || !r->sin) return {ELMH_ERR_ARG, "null rotary table"};
+  if (r->max_pos < 1) return {ELMH_ERR_ARG, "rotary table without positions"};
+  if (r->rot_dim < 2 || r->rot_dim % 2 || r->rot_dim > head_dim) return {ELMH_ERR_ARG, "rot_dim: even, 2 .. head_dim"};
+  if (r->interleaved != 0 && r->interleaved != 1) return {ELMH_ERR_ARG, "interleaved: 0 or 1"};
+  return {};
+}
+
+inline PagedFault check_table(const int32_t* table, int n_seqs, int max_pages, int page_size) {
+  if (!table) return {ELMH_ERR_ARG, "null page table"};
+  if (n_seqs < 1 || max_pages < 1) return {ELMH_ERR_ARG, "n_seqs and max_pages are at least 1"};
+  if ((int64_t)max_pages * page_size > INT32_MAX) return {ELMH_ERR_ARG, "max_pages * page_size past 2^31 - 1 positions"};
+  return {};
+}
+
+// n rows of n_kv heads: strides in values, 0 for the contiguous [n][n_kv][head_dim]
+struct RowStrides {
+  int64_t row = 0, head = 0;
+};
+inline RowStrides row_strides(int64_t row, int64_t head, int n_kv, int head_dim) {
+  return {row ? row : (int64_t)n_kv * head_dim, head ? head : (int64_t)head_dim};
+}
+// written: the rows go to memory, so no two of them may share a value
+inline PagedFault check_rows(int64_t n, int64_t row, int64_t head, int n_kv, int head_dim, bool written) {
+  if (n < 1 || n > (int64_t(1) << 24)) return {ELMH_ERR_ARG, "rows outside 1 .. 2^24"};
+  constexpr int64_t most = int64_t(1) << 40;
+  if (row < 0 || head < 0 || row > most || head > most) return {ELMH_ERR_ARG, "row and head strides: 0 .. 2^40"};
+  const RowStrides s = row_strides(row, head, n_kv, head_dim);
+  const bool rows_apart = (n == 1 || s.row >= (n_kv - 1) * s.head + head_dim) && (n_kv == 1 || s.head >= head_dim);
+  const bool heads_apart = (n_kv == 1 || s.head >= (n - 1) * s.row + head_dim) && (n == 1 || s.row >= head_dim);
+  if (written && !rows_apart && !heads_apart) return {ELMH_ERR_ARG, "strides at which rows overlap"};
+  return {};
+}
+
+inline PagedFault check_paged_rows(const float* k, const float* v, int64_t n, int64_t row, int64_t head,
+                                   const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages,
+                                   const int32_t* pos, const int32_t* seq, const elmh_rope* rope, bool written) {
+  if (!k || !v) return {ELMH_ERR_ARG, "null keys or values"};
+  PagedFault f = check_kv_pages(pages);
+  if (!f.code) f = check_table(table, n_seqs, max_pages, pages->page_size);
+  if (!f.code) f = check_rows(n, row, head, pages->n_kv, pages->head_dim, written);
+  if (!f.code) f = check_rope(rope, pages->head_dim);
+  if (f.code) return f;
+  if (!pos) return {ELMH_ERR_ARG, "null positions"};
+  if (!seq && n > n_seqs) return {ELMH_ERR_ARG, "without seq, row i is of sequence i: n <= n_seqs"};
+  return {};
+}
+
+inline PagedFault check_paged_attention(const float* q, const float* out, int64_t q_row, int n_heads,
+                                        const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages,
+                                        const int32_t* lens, int max_len, const elmh_rope* rope) {
+  if (!q || !out || !lens) return {ELMH_ERR_ARG, "null q, out or lens"};
+  PagedFault f = check_kv_pages(pages);
+  if (!f.code) f = check_table(table, n_seqs, max_pages, pages->page_size);
+  if (!f.code) f = check_rope(rope, pages->head_dim);
+  if (f.code) return f;
+  if (q == out) return {ELMH_ERR_ARG, "out may not overlap q"};
+  if (n_heads < 1 || n_heads % pages->n_kv || n_heads / pages->n_kv > 256)
+    return {ELMH_ERR_ARG, "n_heads: a multiple of the kv heads, at most 256 of each"};
+  if (n_seqs > 65535) return {ELMH_ERR_ARG, "at most 65535 sequences a call"};
+  if (q_row < 0 || q_row > (int64_t(1) << 40)) return {ELMH_ERR_ARG, "q_row: 0 .. 2^40"};
+  if (max_len < 1 || max_len > (int64_t)max_pages * pages->page_size)
+    return {ELMH_ERR_ARG, "max_len: 1 .. max_pages * page_size"};
+  if (rope && max_len > rope->max_pos) return {ELMH_ERR_ARG, "max_len past the rotary table"};
+  return {};
+}
+
+inline PagedFault check_rope_rows(const float* x, const float* y, int64_t T, int n_heads, int head_dim, int64_t x_row,
+                                  int64_t y_row, const elmh_rope* rope, const int32_t* pos, int64_t pos0) {
+  if (!x || !y || !rope) return {ELMH_ERR_ARG, "null x, y or rope"};
+  if (T < 1 || T > (int64_t(1) << 24) || n_heads < 1 || n_heads > 4096) return {ELMH_ERR_ARG, "rows 1 .. 2^24, heads 1 .. 4096"};
+  if (head_dim < 2 || head_dim > 1024 || head_dim % 2) return {ELMH_ERR_ARG, "head_dim: even, 2 .. 1024"};
+  const PagedFault f = check_rope(rope, head_dim);
+  if (f.code) return f;
+  const int64_t width = (int64_t)n_heads * head_dim;
+  if (x_row < 0 || y_row < 0 || x_row > (int64_t(1) << 40) || y_row > (int64_t(1) << 40))
+    return {ELMH_ERR_ARG, "row strides: 0 .. 2^40"};
+  if (T > 1 && y_row && y_row < width) return {ELMH_ERR_ARG, "y's rows overlap"};
+  if (x == y && T > 1 && (x_row ? x_row : width) != (y_row ? y_row : width))
+    return {ELMH_ERR_ARG, "in place: x and y have one stride"};
+  if (!pos && (pos0 < 0 || pos0 + T > rope->max_pos)) return {ELMH_ERR_ARG, "positions past the rotary table"};
+  return {};
+}
+
+inline PagedFault check_rope_table(const float* c, const float* s, int64_t pos0, int64_t n, int rot_dim, double theta,
+                                   const elmh_rope_scaling* sc) {
+  if (!c || !s) return {ELMH_ERR_ARG, "null cos or sin"};
+  if (pos0 < 0 || n < 1 || pos0 > INT32_MAX || n > INT32_MAX || pos0 + n > INT32_MAX)
+    return {ELMH_ERR_ARG, "positions 0 .. 2^31 - 2, at least one"};
+  if (rot_dim < 2 || rot_dim % 2 || rot_dim > 1024) return {ELMH_ERR_ARG, "rot_dim: even, 2 .. 1024"};
+  if (!(theta > 1.0) || !std::isfinite(theta)) return {ELMH_ERR_ARG, "theta: above 1 and finite"};
+  if (!sc) return {};
+  if (sc->kind != ELMH_ROPE_LINEAR && sc->kind != ELMH_ROPE_BANDS && sc->kind != ELMH_ROPE_YARN)
+    return {ELMH_ERR_UNSUPPORTED, "scaling: linear, bands and yarn are known"};
+  if (!(sc->factor >= 1.0) || !std::isfinite(sc->factor)) return {ELMH_ERR_ARG, "scaling factor: at least 1 and finite"};
+  if (!(sc->magnitude > 0.0) || !std::isfinite(sc->magnitude)) return {ELMH_ERR_ARG, "magnitude: above 0 and finite"};
+  if (sc->kind == ELMH_ROPE_LINEAR) return {};
+  if (!(sc->orig_ctx >= 1.0) || !std::isfinite(sc->orig_ctx)) return {ELMH_ERR_ARG, "orig_ctx: at least 1 and finite"};
+  if (!(sc->low > 0.0) || !(sc->high > sc->low) || !std::isfinite(sc->high)) return {ELMH_ERR_ARG, "low and high turns: 0 < low < high"};
+  return {};
+}
+
+// ---------------------------------------------------------------- scaled rotary frequencies
+
+// How the pair i's frequency f = theta^(-2 i / rot) is changed, as numbers that do not depend on i
+struct RopeBand {
+  int kind = 0;            // 0: none
+  double factor = 1, magnitude = 1;
+  double a = 0, b = 1;     // bands: keep = clamp(f * a - b); yarn: keep = 1 - clamp((i - a) * b)
+};
+inline RopeBand rope_band(int rot_dim, double theta, const elmh_rope_scaling* sc) {
+  RopeBand r;
+  if (!sc) return r;
+  constexpr double kTwoPi = 6.283185307179586476925;
+  r.kind = sc->kind;
+  r.factor = sc->factor;
+  r.magnitude = sc->magnitude;
+  if (sc->kind == ELMH_ROPE_BANDS) {
+    r.a = sc->orig_ctx / kTwoPi / (sc->high - sc->low);
+    r.b = sc->low / (sc->high - sc->low);
+  } else if (sc->kind == ELMH_ROPE_YARN) {
+    // the (fractional) pair index that makes t turns over orig_ctx
+    const auto pair = [&](double t) { return rot_dim * std::log(sc->orig_ctx / (kTwoPi * t)) / (2 * std::log(theta)); };
+    const double lo = std::fmax(std::floor(pair(sc->high)), 0.0), hi = std::fmin(std::ceil(pair(sc->low)), rot_dim - 1.0);
+    r.a = lo;
+    r.b = 1.0 / std::fmax(hi - lo, 0.001);
+  }
+  return r;
+}
+ELM_HD double rope_scaled(const RopeBand& r, double f, int i) {
+  if (r.kind == 0) return f;
+  if (r.kind == ELMH_ROPE_LINEAR) return f / r.factor;
+  double keep = r.kind == ELMH_ROPE_BANDS ? f * r.a - r.b : 1.0 - (i - r.a) * r.b;
+  keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+  return f * (keep + (1.0 - keep) / r.factor);
+}
+
+}  // namespace elmh

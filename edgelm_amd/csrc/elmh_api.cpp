@@ -56,6 +56,8 @@ struct elmh_ctx {
   DevBuf nrm;
   // attention score rows longer than LDS holds
   DevBuf asc;
+  // paged attention: the parts of split sequences
+  DevBuf pat;
   // FFN pairs (elmh_ffn_dev): h quantized by the SwiGLU launch for the down projection
   DevBuf hq, hd, hs;
   // bumped whenever a scratch buffer above moves (a graph captured before then holds stale addresses)
@@ -731,7 +733,7 @@ void elmh_destroy(elmh_ctx* c) {
   if (!c) return;
   DeviceGuard g(c);
   (void)hipStreamSynchronize(c->stream);
-  for (DevBuf* b : {&c->x, &c->y, &c->res, &c->xq, &c->xd, &c->xs, &c->gu, &c->nrm, &c->asc, &c->hq, &c->hd, &c->hs})
+  for (DevBuf* b : {&c->x, &c->y, &c->res, &c->xq, &c->xd, &c->xs, &c->gu, &c->nrm, &c->asc, &c->pat, &c->hq, &c->hd, &c->hs})
     if (b->p) (void)hipFree(b->p);
   if (c->argmax_scratch) (void)hipFree(c->argmax_scratch);
   (void)hipStreamDestroy(c->stream);
@@ -1349,6 +1351,70 @@ int elmh_attention_step_dev(elmh_ctx* c, const float* q, const float* k, const f
     return rc;
   HIP_OR_FAIL(c, launch_attention(q, k, v, out, 1, 0, pos_dev, n_heads, n_kv, head_dim, k_cache, v_cache, max_ctx,
                                   rope_cos, rope_sin, c->stream, nullptr, nullptr, 0, nullptr, gsc));
+  return ELMH_OK;
+}
+
+int elmh_kv_page_bytes(int dtype, int n_kv, int head_dim, int page_size, size_t* data, size_t* scales) {
+  if (!data || !scales) return fail(nullptr, ELMH_ERR_ARG, "kv_page_bytes: null argument");
+  const PagedFault f = check_kv_shape(dtype, n_kv, head_dim, page_size);
+  if (f.code) return fail(nullptr, f.code, "kv_page_bytes: %s", f.what);
+  *data = (size_t)n_kv * page_size * kv_row_bytes(dtype, head_dim);
+  *scales = (size_t)n_kv * page_size * kv_groups(dtype, head_dim) * sizeof(float);
+  return ELMH_OK;
+}
+
+int elmh_rope_table_dev(elmh_ctx* c, float* cs, float* sn, int64_t pos0, int64_t n, int rot_dim, double theta,
+                        const elmh_rope_scaling* scaling) {
+  if (!c) return fail(c, ELMH_ERR_ARG, "rope_table: null ctx");
+  const PagedFault f = check_rope_table(cs, sn, pos0, n, rot_dim, theta, scaling);
+  if (f.code) return fail(c, f.code, "rope_table: %s", f.what);
+  DeviceGuard g(c);
+  HIP_OR_FAIL(c, launch_rope_table(cs, sn, pos0, n, rot_dim, theta, rope_band(rot_dim, theta, scaling), c->stream));
+  return ELMH_OK;
+}
+
+int elmh_rope_dev(elmh_ctx* c, const float* x, float* y, int T, int n_heads, int head_dim, int64_t x_row, int64_t y_row,
+                  const elmh_rope* rope, const int32_t* pos, int64_t pos0) {
+  if (!c) return fail(c, ELMH_ERR_ARG, "rope: null ctx");
+  const PagedFault f = check_rope_rows(x, y, T, n_heads, head_dim, x_row, y_row, rope, pos, pos0);
+  if (f.code) return fail(c, f.code, "rope: %s", f.what);
+  DeviceGuard g(c);
+  HIP_OR_FAIL(c, launch_rope(x, y, T, n_heads, head_dim, x_row, y_row, *rope, pos, pos0, c->stream));
+  return ELMH_OK;
+}
+
+int elmh_paged_append_dev(elmh_ctx* c, const float* k, const float* v, int n, int64_t row, int64_t head,
+                          const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages, const int32_t* pos,
+                          const int32_t* seq, const elmh_rope* rope) {
+  if (!c) return fail(c, ELMH_ERR_ARG, "paged_append: null ctx");
+  const PagedFault f = check_paged_rows(k, v, n, row, head, pages, table, n_seqs, max_pages, pos, seq, rope, false);
+  if (f.code) return fail(c, f.code, "paged_append: %s", f.what);
+  DeviceGuard g(c);
+  HIP_OR_FAIL(c, launch_paged_append(k, v, n, row, head, *pages, table, n_seqs, max_pages, pos, seq, rope, c->stream));
+  return ELMH_OK;
+}
+
+int elmh_paged_read_dev(elmh_ctx* c, float* k, float* v, int n, int64_t row, int64_t head, const elmh_kv_pages* pages,
+                        const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq) {
+  if (!c) return fail(c, ELMH_ERR_ARG, "paged_read: null ctx");
+  const PagedFault f = check_paged_rows(k, v, n, row, head, pages, table, n_seqs, max_pages, pos, seq, nullptr, true);
+  if (f.code) return fail(c, f.code, "paged_read: %s", f.what);
+  DeviceGuard g(c);
+  HIP_OR_FAIL(c, launch_paged_read(k, v, n, row, head, *pages, table, n_seqs, max_pages, pos, seq, c->stream));
+  return ELMH_OK;
+}
+
+int elmh_paged_attention_dev(elmh_ctx* c, const float* q, float* out, int64_t q_row, int n_heads,
+                             const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages,
+                             const int32_t* lens, int max_len, const elmh_rope* rope) {
+  if (!c) return fail(c, ELMH_ERR_ARG, "paged_attention: null ctx");
+  const PagedFault f = check_paged_attention(q, out, q_row, n_heads, pages, table, n_seqs, max_pages, lens, max_len, rope);
+  if (f.code) return fail(c, f.code, "paged_attention: %s", f.what);
+  DeviceGuard g(c);
+  const int parts = paged_attention_parts(n_seqs, n_heads, pages->n_kv, max_len);
+  if (const int rc = ensure(c, c->pat, paged_attention_scratch_bytes(n_seqs, n_heads, pages->head_dim, parts))) return rc;
+  HIP_OR_FAIL(c, launch_paged_attention(q, out, q_row, n_heads, *pages, table, n_seqs, max_pages, lens, max_len, rope, parts,
+                                        static_cast<float*>(c->pat.p), c->stream));
   return ELMH_OK;
 }
 

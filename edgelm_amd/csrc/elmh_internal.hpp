@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "elm_device_once.h"
+#include "elm_paged.h"
 #include "elm_routes.h"
 
 namespace elmh {
@@ -210,6 +211,23 @@ hipError_t launch_argmax_parts(const float* x, int64_t n, int32_t* out, int32_t*
 // Measurement: `blocks` 256-thread workgroups of the rescale-ceiling kernel (mode 0 MFMA only, 1 q8 exact
 // rescale, 2 q4 exact rescale), `iters` blocks per wave; sink: blocks * 256 floats.
 hipError_t launch_rescale_ceiling(int mode, int blocks, int iters, float* sink, hipStream_t s);
+// ---------------------------------------------------------------- launchers (elmh_paged.hip; arguments checked by elm_paged.h)
+hipError_t launch_rope_table(float* cs, float* sn, int64_t pos0, int64_t n, int rot_dim, double theta, const RopeBand& band,
+                             hipStream_t s);
+hipError_t launch_rope(const float* x, float* y, int T, int n_heads, int hd, int64_t x_row, int64_t y_row,
+                       const elmh_rope& rope, const int32_t* pos, int64_t pos0, hipStream_t s);
+hipError_t launch_paged_append(const float* k, const float* v, int n, int64_t row, int64_t head, const elmh_kv_pages& pages,
+                               const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq,
+                               const elmh_rope* rope, hipStream_t s);
+hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t head, const elmh_kv_pages& pages,
+                             const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq,
+                             hipStream_t s);
+// Parts a sequence is split into at most, and the scratch that the parts need (0 for one part)
+int paged_attention_parts(int n_seqs, int n_heads, int n_kv, int max_len);
+size_t paged_attention_scratch_bytes(int n_seqs, int n_heads, int head_dim, int parts);
+hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int n_heads, const elmh_kv_pages& pages,
+                                  const int32_t* table, int n_seqs, int max_pages, const int32_t* lens, int max_len,
+                                  const elmh_rope* rope, int parts, float* scratch, hipStream_t s);
 // Test hook: S[t][n][b] for pre-quantized row-major activations.
 hipError_t launch_block_sums(const DevWeight& w, const int8_t* xq, int T, int32_t* S, hipStream_t s);
 

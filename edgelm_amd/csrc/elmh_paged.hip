@@ -1,0 +1,877 @@
+// Many sequences over one paged key/value cache: rotary tables and rotation, rows written into pages (quantized) and read
+// back, and the attention of one new token a sequence. The layout of the pools is in include/elmh.h.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "elm_dpp.h"
+#include "elm_paged.h"
+#include "elm_quant.h"
+#include "elmh_internal.hpp"
+
+namespace elmh {
+namespace {
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+// ---------------------------------------------------------------- rotary tables and rotation
+
+__global__ __launch_bounds__(256) void rope_table_kernel(float* __restrict__ cs, float* __restrict__ sn, int64_t pos0,
+                                                         int64_t n, int half, double theta, RopeBand band) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= n * half) return;
+  const int i = (int)(at % half);
+  const double f = rope_scaled(band, pow(theta, -2.0 * i / (2 * half)), i);
+  const double a = (double)(pos0 + at / half) * f;
+  cs[at] = (float)(cos(a) * band.magnitude);
+  sn[at] = (float)(sin(a) * band.magnitude);
+}
+
+// One thread a pair: (i, i + rot / 2) or (2 i, 2 i + 1), and past the rotated part two neighbours that pass.
+__global__ __launch_bounds__(256) void rope_kernel(const float* x, float* y, int64_t pairs, int n_heads, int hd,
+                                                   int64_t x_row, int64_t y_row, const float* __restrict__ cs,
+                                                   const float* __restrict__ sn, int max_pos, int rot, int inter,
+                                                   const int32_t* __restrict__ pos, int64_t pos0) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= pairs) return;
+  const int i = (int)(at % (hd / 2)), half = rot / 2;
+  const int64_t row = at / (hd / 2), t = row / n_heads;
+  const int64_t p = pos ? pos[t] : pos0 + t;
+  if (p < 0 || p >= max_pos) return;
+  const int64_t head = (row % n_heads) * hd;
+  const bool turned = i < half;
+  const int a = turned && !inter ? i : 2 * i, b = turned && !inter ? i + half : 2 * i + 1;
+  float u = x[t * x_row + head + a], v = x[t * x_row + head + b];
+  if (turned) {
+    const float c = cs[p * half + i], s = sn[p * half + i];
+    const float u0 = u;
+    u = u0 * c - v * s;
+    v = v * c + u0 * s;
+  }
+  y[t * y_row + head + a] = u;
+  y[t * y_row + head + b] = v;
+}
+
+// ---------------------------------------------------------------- rows into pages and back
+
+struct RowArgs {
+  const float *k, *v;  // rows in (append)
+  float *ko, *vo;      // rows out (read)
+  int64_t row, head;
+  int n;
+  elmh_kv_pages pages;
+  const int32_t* table;
+  int n_seqs, max_pages;
+  const int32_t *pos, *seq;
+  const float *cs, *sn;
+  int max_pos, rot, inter;
+};
+
+// Where row i of a call lies in the cache; page < 0: the row is skipped
+struct RowPlace {
+  int64_t page;
+  int slot, pos;
+};
+__device__ __forceinline__ RowPlace row_place(const RowArgs& a, int i) {
+  const int pos = a.pos[i], seq = a.seq ? a.seq[i] : i;
+  if (seq < 0 || seq >= a.n_seqs || pos < 0 || (a.cs && pos >= a.max_pos)) return {-1, 0, 0};
+  const int ps = a.pages.page_size;
+  return {kv_page_of(a.table + (int64_t)seq * a.max_pages, a.max_pages, a.pages.n_pages, pos, ps), pos % ps, pos};
+}
+
+// Value d of a head's row x, rotated
+__device__ __forceinline__ float rotated(const float* x, int d, const float* cs, const float* sn, int half, int inter) {
+  if (d >= 2 * half) return x[d];
+  const int i = inter ? d >> 1 : d < half ? d : d - half;
+  const bool second = inter ? d & 1 : d >= half;
+  const float c = cs[i], s = sn[i], self = x[d];
+  const float other = x[inter ? d ^ 1 : second ? d - half : d + half];
+  return second ? self * c + other * s : self * c - other * s;
+}
+
+// Lanes that share a row, eight values each: head_dim / 8 rounded up to a power of two (the rest idle)
+ELM_HD int row_lanes(int hd) { return hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
+
+__global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
+  const elmh_kv_pages& pg = a.pages;
+  const int hd = pg.head_dim, lanes = row_lanes(hd);
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int c = threadIdx.x % lanes, d0 = 8 * c;
+  const bool keys = blockIdx.y == 0, in = at < (int64_t)a.n * pg.n_kv && d0 < hd;
+  const int t = (int)(at / pg.n_kv), h = (int)(at % pg.n_kv);
+  RowPlace w{-1, 0, 0};
+  if (in) w = row_place(a, t);
+  const bool live = w.page >= 0;
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  if (live) {
+    const float* src = (keys ? a.k : a.v) + t * a.row + h * a.head;
+    const int half = a.rot / 2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x[e] = keys && a.cs ? rotated(src, d0 + e, a.cs + (int64_t)w.pos * half, a.sn + (int64_t)w.pos * half, half, a.inter)
+                          : src[d0 + e];
+  }
+  const int64_t row = live ? kv_row(w.page, h, w.slot, pg.n_kv, pg.page_size) : 0;
+  void* pool = keys ? pg.k : pg.v;
+  float* scales = keys ? pg.k_scale : pg.v_scale;
+  if (pg.dtype == ELMH_Q8) {
+    float amax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+    for (int off = lanes / 2; off; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
+    const float s = amax / 127.f;
+    int q[8];
+    elm_q8_group<8>(x, s == 0.f ? 1.f : s, q);
+    if (!live) return;
+    u32x2 b{0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e / 4] |= (uint32_t)(q[e] & 0xFF) << (8 * (e % 4));
+    *reinterpret_cast<u32x2*>(static_cast<int8_t*>(pool) + row * hd + d0) = b;
+    if (c == 0) scales[row] = s;
+    return;
+  }
+  if (pg.dtype == ELMH_Q4) {
+    // the group's first value of largest magnitude: in this lane, then over the four lanes of the group
+    float m = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m = fabsf(x[e]) > fabsf(m) ? x[e] : m;
+#pragma unroll
+    for (int off = 1; off <= 2; off <<= 1) {
+      const float o = __shfl_xor(m, off, 64);
+      const bool lower = c & off;  // the other lane's values come first
+      m = lower ? (fabsf(o) >= fabsf(m) ? o : m) : (fabsf(o) > fabsf(m) ? o : m);
+    }
+    const float s = m / -8.f, div = s == 0.f ? 1.f : s;
+    if (!live) return;
+    uint32_t nib[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float r = x[e] / div;
+      nib[e] = (uint32_t)((int)fminf(7.f, fmaxf(-8.f, copysignf(floorf(fabsf(r) + 0.5f), r))) + 8);
+    }
+    uint8_t* dst = static_cast<uint8_t*>(pool) + row * (hd / 2);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+      dst[keys ? q4_key_byte(d0 + e, hd) : q4_value_byte(d0 + e, hd)] = (uint8_t)(nib[e] | nib[e + 1] << 4);
+    if (c % 4 == 0) scales[kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, hd / 32) + (int64_t)(c / 4) * pg.page_size] = s;
+    return;
+  }
+  if (!live) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (pg.dtype == ELMH_F32)
+      static_cast<float*>(pool)[row * hd + d0 + e] = x[e];
+    else if (pg.dtype == ELMH_F16)
+      static_cast<_Float16*>(pool)[row * hd + d0 + e] = (_Float16)x[e];
+    else
+      static_cast<__bf16*>(pool)[row * hd + d0 + e] = (__bf16)x[e];
+  }
+}
+
+__global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a) {
+  const elmh_kv_pages& pg = a.pages;
+  const int hd = pg.head_dim, lanes = row_lanes(hd);
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int c = threadIdx.x % lanes, d0 = 8 * c;
+  if (at >= (int64_t)a.n * pg.n_kv || d0 >= hd) return;
+  const bool keys = blockIdx.y == 0;
+  const int t = (int)(at / pg.n_kv), h = (int)(at % pg.n_kv);
+  const RowPlace w = row_place(a, t);
+  if (w.page < 0) return;
+  const int64_t row = kv_row(w.page, h, w.slot, pg.n_kv, pg.page_size);
+  const void* pool = keys ? pg.k : pg.v;
+  const float* scales = keys ? pg.k_scale : pg.v_scale;
+  float* dst = (keys ? a.ko : a.vo) + t * a.row + h * a.head + d0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float x;
+    if (pg.dtype == ELMH_F32) {
+      x = static_cast<const float*>(pool)[row * hd + d0 + e];
+    } else if (pg.dtype == ELMH_F16) {
+      x = (float)static_cast<const _Float16*>(pool)[row * hd + d0 + e];
+    } else if (pg.dtype == ELMH_BF16) {
+      x = (float)static_cast<const __bf16*>(pool)[row * hd + d0 + e];
+    } else if (pg.dtype == ELMH_Q8) {
+      x = (float)static_cast<const int8_t*>(pool)[row * hd + d0 + e] * scales[row];
+    } else {
+      const int d = d0 + e;
+      const int b = static_cast<const uint8_t*>(pool)[row * (hd / 2) + (keys ? q4_key_byte(d & ~1, hd) : q4_value_byte(d & ~1, hd))];
+      x = (float)((d & 1 ? b >> 4 : b & 15) - 8) *
+          scales[kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, hd / 32) + (int64_t)(d / 32) * pg.page_size];
+    }
+    dst[e] = x;
+  }
+}
+
+// ---------------------------------------------------------------- attention of one new token a sequence
+
+constexpr int kPaWaves = 4;
+constexpr int kPaHeads = 16;       // query heads a workgroup takes: the columns of a 16 x 16 tile
+constexpr int kPaLeastUnits = 4;   // of a part: one unit a wave
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// The matrix instructions take 16-bit operands, 32 values deep, or f32 ones, 4 deep. Products are exact in both (f32
+// accumulation); what is in 32 bits (queries, softmax weights) is split into 16-bit pieces whose sum has its 24 bits:
+//   f16, q8, q4 caches: f16 operands (levels are exact in f16), two pieces of 11 bits, a power of two taken out first;
+//   bf16 caches: bf16 operands, three pieces of 8 bits.
+enum { kOpF32 = 0, kOpF16 = 1, kOpBF16 = 2 };
+constexpr int op_of(int dt) { return dt == ELMH_F32 ? kOpF32 : dt == ELMH_BF16 ? kOpBF16 : kOpF16; }
+constexpr int pieces_of(int dt) { return dt == ELMH_BF16 ? 3 : 2; }
+
+template <int OP>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (OP == kOpBF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// x[0..7] as the pieces of a 32-deep operand. f16: |x| < 2^15.
+template <int OP>
+__device__ __forceinline__ void split8(const float* x, u32x4* out) {
+  if constexpr (OP == kOpF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto p = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
+      const f16x2 r{(_Float16)(x[2 * i] - (float)p[0]), (_Float16)(x[2 * i + 1] - (float)p[1])};
+      out[0][i] = __builtin_bit_cast(uint32_t, p);
+      out[1][i] = __builtin_bit_cast(uint32_t, r);
+    }
+  } else {  // the top 16 bits, twice, and what is left: exact
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t u[2][3];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = x[2 * i + e];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          u[e][k] = __float_as_uint(v);
+          v -= __uint_as_float(u[e][k] & 0xFFFF0000u);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) out[k][i] = __builtin_amdgcn_perm(u[1][k], u[0][k], 0x07060302);
+    }
+  }
+}
+
+// int8 levels as f16: the byte u = q + 128 under the exponent of 1024 is 1024 + u, minus 1152 gives q. w: pairs of bytes in the
+// low halves' low bytes.
+__device__ __forceinline__ uint32_t f16_add(uint32_t w, float add) {
+  const f16x2 v = __builtin_bit_cast(f16x2, w) + f16x2{(_Float16)add, (_Float16)add};
+  return __builtin_bit_cast(uint32_t, v);
+}
+// nibbles n at bits 0-3 of each half: 1024 + n - 1032; at bits 4-7: (1024 + 16 n) / 16 - 72
+__device__ __forceinline__ uint32_t f16_low_nibbles(uint32_t w) { return f16_add((w & 0x000F000Fu) | 0x64006400u, -1032.f); }
+__device__ __forceinline__ uint32_t f16_high_nibbles(uint32_t w) {
+  const f16x2 v = __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u);
+  const f16x2 r = __builtin_elementwise_fma(v, f16x2{(_Float16)0.0625f, (_Float16)0.0625f}, f16x2{(_Float16)-72.f, (_Float16)-72.f});
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+// ---- which values of a row a lane holds. Lane = 16 g + n.
+// Keys (rows of the 16 x 32 operand are tokens, n): step j's eight values of lane group g.
+template <int DT, int NB>
+ELM_HD constexpr int key_dim(int j, int g, int e) {
+  if (DT == ELMH_Q8 && !(NB % 2 == 1 && j == NB - 1)) return 64 * (j / 2) + 16 * g + 8 * (j % 2) + e;
+  if (DT == ELMH_Q4) return 32 * j + 8 * g + (e / 2) + 4 * (e % 2);
+  return 32 * j + 8 * g + e;
+}
+// Values (rows of the operand are the row's values, 16 of them an instruction): value x (0 .. 2 NB - 1) of lane n. A lane's
+// values are neighbours in units of 32 values times 4, 2 or 1, so that sixteen lanes read a unit as one piece.
+constexpr int unit_width(int NB, int x) {  // of the unit that value x is in
+  int left = NB, at = 0;
+  while (true) {
+    const int w = left >= 4 ? 4 : left >= 2 ? 2 : 1;
+    if (x < at + 2 * w) return w;
+    at += 2 * w;
+    left -= w;
+  }
+}
+constexpr int unit_start(int NB, int x) {  // its first value index x
+  int left = NB, at = 0;
+  while (true) {
+    const int w = left >= 4 ? 4 : left >= 2 ? 2 : 1;
+    if (x < at + 2 * w) return at;
+    at += 2 * w;
+    left -= w;
+  }
+}
+template <int DT, int NB>
+__device__ __forceinline__ constexpr int value_dim(int x, int n) {
+  if (DT == ELMH_Q4) return 32 * (x / 2) + 2 * n + x % 2;
+  const int w = unit_width(NB, x), s = unit_start(NB, x);
+  return 16 * s + 2 * w * n + (x - s);
+}
+
+// ---- a block of 16 tokens' rows in registers, as loaded
+constexpr int key_words(int dt, int NB) { return dt == ELMH_F32 ? 8 * NB : dt == ELMH_Q8 ? 2 * NB : dt == ELMH_Q4 ? NB : 4 * NB; }
+constexpr int value_words(int dt, int NB) {  // per token (four tokens a lane)
+  return dt == ELMH_F32 ? 2 * NB : dt == ELMH_Q8 ? (NB + 1) / 2 : dt == ELMH_Q4 ? (NB + 3) / 4 : NB;
+}
+
+template <int WORDS>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (WORDS >= 4) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = v[i];
+    if constexpr (WORDS > 4) load_words<WORDS - 4>(p + 16, w + 4);
+  } else if constexpr (WORDS >= 2) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    w[0] = v[0];
+    w[1] = v[1];
+    if constexpr (WORDS > 2) load_words<WORDS - 2>(p + 8, w + 2);
+  } else if constexpr (WORDS == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// row: this lane's token's key row
+template <int DT, int NB>
+__device__ __forceinline__ void load_key(const uint8_t* row, int g, uint32_t (&w)[key_words(DT, NB)]) {
+  if constexpr (DT == ELMH_F32) {
+#pragma unroll
+    for (int j = 0; j < 2 * NB; ++j) load_words<4>(row + 64 * j + 16 * g, w + 4 * j);
+  } else if constexpr (DT == ELMH_Q8) {
+#pragma unroll
+    for (int j = 0; j + 1 < NB; j += 2) load_words<4>(row + 32 * j + 16 * g, w + 2 * j);
+    if constexpr (NB % 2) load_words<2>(row + 32 * (NB - 1) + 8 * g, w + 2 * (NB - 1));
+  } else if constexpr (DT == ELMH_Q4) {
+    if constexpr (NB == 3) {  // 12 g: not on 8 bytes
+#pragma unroll
+      for (int j = 0; j < NB; ++j) w[j] = *reinterpret_cast<const uint32_t*>(row + 12 * g + 4 * j);
+    } else if constexpr (NB == 6) {  // 24 g: on 8
+#pragma unroll
+      for (int j = 0; j < NB; j += 2) load_words<2>(row + 24 * g + 4 * j, w + j);
+    } else {
+      load_words<NB>(row + 4 * NB * g, w);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) load_words<4>(row + 64 * j + 16 * g, w + 4 * j);
+  }
+}
+// the operand of step j (16-bit forms)
+template <int DT, int NB>
+__device__ __forceinline__ u32x4 key_operand(const uint32_t (&w)[key_words(DT, NB)], int j) {
+  if constexpr (DT == ELMH_Q8) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t u = w[2 * j + i] ^ 0x80808080u;
+      o[2 * i] = f16_add(__builtin_amdgcn_perm(u, 0x64646464u, 0x00050004), -1152.f);
+      o[2 * i + 1] = f16_add(__builtin_amdgcn_perm(u, 0x64646464u, 0x00070006), -1152.f);
+    }
+    return o;
+  } else if constexpr (DT == ELMH_Q4) {
+    const uint32_t u = w[j], v = u >> 8;
+    return u32x4{f16_low_nibbles(u), f16_high_nibbles(u), f16_low_nibbles(v), f16_high_nibbles(v)};
+  } else {
+    return u32x4{w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]};
+  }
+}
+
+// row: a token's value row; lane n's part of it
+template <int DT, int NB>
+__device__ __forceinline__ void load_value(const uint8_t* row, int n, uint32_t (&w)[value_words(DT, NB)]) {
+  if constexpr (DT == ELMH_Q4) {  // NB bytes at n * NB
+    if constexpr (NB == 1) {
+      w[0] = row[n];
+    } else if constexpr (NB == 2) {
+      w[0] = *reinterpret_cast<const uint16_t*>(row + 2 * n);
+    } else if constexpr (NB == 3) {
+      w[0] = row[3 * n] | row[3 * n + 1] << 8 | row[3 * n + 2] << 16;
+    } else if constexpr (NB == 6) {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(row + 6 * n);
+      w[0] = p[0] | (uint32_t)p[1] << 16;
+      w[1] = p[2];
+    } else {
+      load_words<NB / 4>(row + NB * n, w);
+    }
+  } else {
+    constexpr int B = DT == ELMH_F32 ? 4 : DT == ELMH_Q8 ? 1 : 2;
+    // units of 4, 2 and 1 times 32 values
+    if constexpr (NB >= 4) load_words<2 * B>(row + 8 * B * n, w);
+    if constexpr (NB == 8) load_words<2 * B>(row + 128 * B + 8 * B * n, w + 2 * B);
+    constexpr int done = NB / 4 * 4;
+    if constexpr ((NB & 2) != 0) load_words<B>(row + 32 * done * B + 4 * B * n, w + done * B / 2);
+    constexpr int last = NB & ~1;
+    if constexpr ((NB & 1) != 0) {
+      const uint8_t* p = row + 32 * last * B + 2 * B * n;
+      if constexpr (B == 1) w[last / 2] = *reinterpret_cast<const uint16_t*>(p);
+      else load_words<B / 2>(p, w + last * B / 2);
+    }
+  }
+}
+// The operand of value x over eight tokens: v[0..3] the first block's, v[4..7] the second's
+template <int DT, int NB>
+__device__ __forceinline__ u32x4 value_operand(const uint32_t (&v)[8][value_words(DT, NB)], int x) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == ELMH_Q8) {
+      const uint32_t a = v[2 * i][x / 4], b = v[2 * i + 1][x / 4];
+      const uint32_t sel = 0x0C040C00u + (x % 4) * 0x00010001u;
+      o[i] = f16_add(__builtin_amdgcn_perm(b, a, sel) | 0x64006400u, -1152.f);  // the bytes were loaded and flipped
+    } else if constexpr (DT == ELMH_Q4) {
+      const int j = x / 2;
+      const uint32_t sel = 0x0C040C00u + (j % 4) * 0x00010001u;
+      const uint32_t w = __builtin_amdgcn_perm(v[2 * i + 1][j / 4], v[2 * i][j / 4], sel);
+      o[i] = x % 2 ? f16_high_nibbles(w) : f16_low_nibbles(w);
+    } else {
+      o[i] = __builtin_amdgcn_perm(v[2 * i + 1][x / 2], v[2 * i][x / 2], x % 2 ? 0x07060302u : 0x05040100u);
+    }
+  }
+  return o;
+}
+
+struct PagedAttnArgs {
+  const float* q;
+  float* out;
+  int64_t q_row;
+  int n_heads, group, head_tiles;  // query heads; per kv head; workgroups a kv head's take
+  elmh_kv_pages pages;
+  const int32_t* table;
+  int max_pages;
+  const int32_t* lens;
+  int max_len;
+  const float *cs, *sn;
+  int rot, inter;
+  int parts;      // a sequence is split into at most
+  float* part_o;  // [seq][head][part][head_dim], unnormalized
+  float* part_s;  // [seq][head][part][2]: running maximum (base 2), sum
+};
+
+__device__ __forceinline__ float max_over_groups(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+// One workgroup: one part of one sequence's cache for up to 16 query heads of one kv head, its waves taking 32 tokens at a time.
+// Scores as K Q^T (tokens x heads) leave a lane with four tokens of one head, which is what the second product V^T P^T takes
+// as its operand: no exchange between lanes but the maximum over the four lane groups. One pass: running maximum m and sum l.
+template <int DT, int NB>
+__global__ __launch_bounds__(64 * kPaWaves) void paged_attention_kernel(PagedAttnArgs a) {
+  constexpr int HD = 32 * NB, OP = op_of(DT), PC = pieces_of(DT);
+  extern __shared__ float lds[];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = blockIdx.x, kvh = blockIdx.y / a.head_tiles, seq = blockIdx.z;
+  const int h0 = kvh * a.group + blockIdx.y % a.head_tiles * kPaHeads;
+  const int heads = min(kPaHeads, (kvh + 1) * a.group - h0);
+  const elmh_kv_pages& pg = a.pages;
+  const int len = min(max(a.lens[seq], 0), a.max_len);
+  const int units = (len + kSplitUnit - 1) / kSplitUnit;
+  const int per = split_size(units, a.parts, kPaLeastUnits), live = split_parts(units, per);
+  float* out = a.out + (int64_t)seq * a.n_heads * HD + (int64_t)h0 * HD;
+  if (len == 0 && part == 0)
+    for (int i = tid; i < heads * HD; i += 64 * kPaWaves) out[i] = 0.f;
+  if (part >= live) return;
+
+  // the queries, rotated at the last position
+  const float* q = a.q + seq * a.q_row + (int64_t)h0 * HD;
+  for (int i = tid; i < heads * HD; i += 64 * kPaWaves) {
+    const int64_t at = (int64_t)(len - 1) * (a.rot / 2);
+    lds[i] = a.cs ? rotated(q + i / HD * HD, i % HD, a.cs + at, a.sn + at, a.rot / 2, a.inter) : q[i];
+  }
+  __syncthreads();
+  // as operands; `scale`: what a product is multiplied by to be a score in units of log2
+  float scale = kLog2e / sqrtf((float)HD);
+  u32x4 qo[OP == kOpF32 ? 1 : NB][OP == kOpF32 ? 1 : PC];
+  float qf[OP == kOpF32 ? 8 * NB : 1];
+  const float* qrow = lds + min(n, heads - 1) * HD;
+  if constexpr (OP == kOpF32) {
+#pragma unroll
+    for (int j = 0; j < 2 * NB; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[4 * j + i] = qrow[16 * j + 4 * g + i];
+  } else {
+    float up = 1.f;
+    if constexpr (OP == kOpF16) {  // the head's largest value to 512 .. 1024: its 24 bits then lie in f16's range
+      float big = 0.f;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qrow[32 * j + 8 * g + e]));
+      big = max_over_groups(big);
+      const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -110), 110);
+      up = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
+      scale *= __uint_as_float((uint32_t)(127 - 9 + ex) << 23);
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = qrow[key_dim<DT, NB>(j, g, e)] * up;
+      split8<OP>(x, qo[j]);
+    }
+  }
+
+  const int32_t* trow = a.table + (int64_t)seq * a.max_pages;
+  const int ps = pg.page_size;
+  constexpr int RB = DT == ELMH_F32 ? 4 * HD : DT == ELMH_Q8 ? HD : DT == ELMH_Q4 ? HD / 2 : 2 * HD;
+  constexpr int NG = DT == ELMH_Q8 ? 1 : DT == ELMH_Q4 ? NB : 0;
+  const uint8_t* kpool = static_cast<const uint8_t*>(pg.k);
+  const uint8_t* vpool = static_cast<const uint8_t*>(pg.v);
+  float m = -INFINITY, l = 0.f;
+  int vexp = -112;  // q8, q4: the softmax weights take the value scales over 2^vexp, the largest seen
+  f32x4 acc[2 * NB];
+#pragma unroll
+  for (int x = 0; x < 2 * NB; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int end = min(units, (part + 1) * per);
+  for (int unit = part * per + wave; unit < end; unit += kPaWaves) {
+    int valid[2];
+    int64_t row[2], srow[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int pos = unit * kSplitUnit + 16 * u;
+      const int64_t page = pos < len ? kv_page_of(trow, a.max_pages, pg.n_pages, pos, ps) : -1;
+      valid[u] = page >= 0 ? min(16, len - pos) : 0;
+      row[u] = kv_row(page >= 0 ? page : 0, kvh, page >= 0 ? pos % ps : 0, pg.n_kv, ps);
+      srow[u] = kv_scale(page >= 0 ? page : 0, kvh, page >= 0 ? pos % ps : 0, pg.n_kv, ps, NG);
+    }
+    const bool whole = valid[0] == 16 && valid[1] == 16;
+
+    float s[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint32_t w[key_words(DT, NB)];
+      load_key<DT, NB>(kpool + (row[u] + n) * RB, g, w);
+      f32x4 sc{0.f, 0.f, 0.f, 0.f};
+      if constexpr (OP == kOpF32) {
+#pragma unroll
+        for (int j = 0; j < 8 * NB; ++j) sc = mfma_f32(__uint_as_float(w[j]), qf[j], sc);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const u32x4 ko = key_operand<DT, NB>(w, j);
+          f32x4 t = DT == ELMH_Q4 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc;
+#pragma unroll
+          for (int p = PC - 1; p >= 0; --p) t = mfma<OP>(ko, qo[j][p], t);
+          if constexpr (DT == ELMH_Q4) {
+            const f32x4 ks = *reinterpret_cast<const f32x4*>(pg.k_scale + srow[u] + (int64_t)j * ps + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[r] = fmaf(t[r], ks[r], sc[r]);
+          } else {
+            sc = t;
+          }
+        }
+      }
+      if constexpr (DT == ELMH_Q8) {
+        const f32x4 ks = *reinterpret_cast<const f32x4*>(pg.k_scale + srow[u] + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[r] *= ks[r];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[4 * u + r] = 4 * g + r < valid[u] ? sc[r] * scale : -INFINITY;
+    }
+
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
+    const float mn = fmaxf(m, max_over_groups(top));
+    const float ref = mn == -INFINITY ? 0.f : mn;  // no token so far: weights of 0, not of exp(-inf + inf)
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+    }
+    float fade = __builtin_amdgcn_exp2f(m - ref);
+    m = mn;
+    l = l * fade + ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+
+    uint32_t v[8][value_words(DT, NB)];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) load_value<DT, NB>(vpool + (row[u] + 4 * g + r) * RB, n, v[4 * u + r]);
+    if constexpr (DT == ELMH_Q8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < value_words(DT, NB); ++k) v[i][k] ^= 0x80808080u;
+    }
+    if constexpr (NG == 0) {  // a slot behind the end may hold a NaN, which a weight of 0 does not remove
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int k = 0; k < value_words(DT, NB); ++k) v[i][k] = 4 * g + i % 4 < valid[i / 4] ? v[i][k] : 0u;
+      }
+    }
+    float vs[NG ? NG : 1][8];
+    if constexpr (NG > 0) {
+      float big = 0.f;
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const f32x4 t = *reinterpret_cast<const f32x4*>(pg.v_scale + srow[u] + (int64_t)j * ps + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            vs[j][4 * u + r] = 4 * g + r < valid[u] ? t[r] : 0.f;
+            big = fmaxf(big, fabsf(vs[j][4 * u + r]));
+          }
+        }
+      if (__any(big > __uint_as_float((uint32_t)(127 + vexp) << 23))) {  // rare after the first tokens
+        const int ex = min((int)(__float_as_uint(wave_max(big)) >> 23) - 126, 120);
+        const int by = min(ex - vexp, 126);
+        fade *= __uint_as_float((uint32_t)(127 - by) << 23);
+        vexp = ex;
+      }
+    }
+    if (__any(fade != 1.f)) {
+#pragma unroll
+      for (int x = 0; x < 2 * NB; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[x][r] *= fade;
+    }
+
+    if constexpr (OP == kOpF32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int x = 0; x < 2 * NB; ++x) acc[x] = mfma_f32(__uint_as_float(v[i][x]), p[i], acc[x]);
+    } else {
+      // f16 pieces: weights up to 2^14, so that a weight 2^-28 of the largest is still a normal number
+      const float up = OP == kOpF16 ? (NG ? __uint_as_float((uint32_t)(127 + 14 - vexp) << 23) : 16384.f) : 1.f;
+      u32x4 po[PC];
+#pragma unroll
+      for (int x = 0; x < 2 * NB; ++x) {
+        if (x == 0 || (DT == ELMH_Q4 && x % 2 == 0)) {
+          float t[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) t[i] = NG ? p[i] * (vs[NG > 1 ? x / 2 : 0][i] * up) : p[i] * up;
+          split8<OP>(t, po);
+        }
+        const u32x4 vo = value_operand<DT, NB>(v, x);
+#pragma unroll
+        for (int k = PC - 1; k >= 0; --k) acc[x] = mfma<OP>(vo, po[k], acc[x]);
+      }
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+
+  // the waves' sums joined: o = sum_w 2^(m_w - M) o_w
+  if constexpr (OP == kOpF16) {
+    const float f = __uint_as_float((uint32_t)(127 + (NG ? vexp : 0) - 14) << 23);
+#pragma unroll
+    for (int x = 0; x < 2 * NB; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[x][r] *= f;
+  }
+  __syncthreads();  // the queries have been read
+  float* stat = lds + kPaWaves * heads * HD;
+  if (n < heads) {
+#pragma unroll
+    for (int x = 0; x < 2 * NB; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) lds[(wave * heads + n) * HD + value_dim<DT, NB>(x, 4 * g + r)] = acc[x][r];
+    if (g == 0) {
+      stat[wave * kPaHeads + n] = m;
+      stat[(kPaWaves + wave) * kPaHeads + n] = l;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < heads * HD; i += 64 * kPaWaves) {
+    const int h = i / HD, d = i % HD;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kPaWaves; ++w) M = fmaxf(M, stat[w * kPaHeads + h]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float o = 0.f, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPaWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(stat[w * kPaHeads + h] - ref);
+      o += f * lds[(w * heads + h) * HD + d];
+      L += f * stat[(kPaWaves + w) * kPaHeads + h];
+    }
+    if (live == 1) {
+      out[i] = L == 0.f ? 0.f : o / L;
+    } else {
+      const int64_t at = ((int64_t)seq * a.n_heads + h0 + h) * a.parts + part;
+      a.part_o[at * HD + d] = o;
+      if (d == 0) {
+        a.part_s[at * 2] = M;
+        a.part_s[at * 2 + 1] = L;
+      }
+    }
+  }
+}
+
+// The parts of a (sequence, head) joined, in their order
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+  const int hd = a.pages.head_dim, d = threadIdx.x, head = blockIdx.x, seq = blockIdx.y;
+  const int len = min(max(a.lens[seq], 0), a.max_len);
+  const int units = (len + kSplitUnit - 1) / kSplitUnit;
+  const int live = split_parts(units, split_size(units, a.parts, kPaLeastUnits));
+  if (live < 2 || d >= hd) return;
+  const int64_t at = ((int64_t)seq * a.n_heads + head) * a.parts;
+  float M = -INFINITY;
+  for (int s = 0; s < live; ++s) M = fmaxf(M, a.part_s[(at + s) * 2]);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float o = 0.f, L = 0.f;
+  for (int s = 0; s < live; ++s) {
+    const float f = __builtin_amdgcn_exp2f(a.part_s[(at + s) * 2] - ref);
+    o += f * a.part_o[(at + s) * hd + d];
+    L += f * a.part_s[(at + s) * 2 + 1];
+  }
+  a.out[((int64_t)seq * a.n_heads + head) * hd + d] = L == 0.f ? 0.f : o / L;
+}
+
+template <int DT, int NB>
+hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, hipStream_t s) {
+  const int heads = a.group < kPaHeads ? a.group : kPaHeads;
+  const size_t lds = (size_t)(kPaWaves * heads * 32 * NB + 2 * kPaWaves * kPaHeads) * sizeof(float);
+  if (lds > 64 * 1024) {
+    static DeviceOnce once;
+    if (!raise_dynamic_lds(once, (const void*)paged_attention_kernel<DT, NB>, 80 * 1024)) return hipErrorInvalidValue;
+  }
+  const dim3 grid(a.parts, a.pages.n_kv * a.head_tiles, n_seqs);
+  paged_attention_kernel<DT, NB><<<grid, 64 * kPaWaves, lds, s>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.parts == 1) return e;
+  paged_join_kernel<<<dim3(a.n_heads, n_seqs), (32 * NB + 63) / 64 * 64, 0, s>>>(a);
+  return hipGetLastError();
+}
+template <int DT>
+hipError_t launch_paged_attention_of(const PagedAttnArgs& a, int n_seqs, hipStream_t s) {
+  switch (a.pages.head_dim) {
+    case 32: return launch_paged_attention_as<DT, 1>(a, n_seqs, s);
+    case 64: return launch_paged_attention_as<DT, 2>(a, n_seqs, s);
+    case 96: return launch_paged_attention_as<DT, 3>(a, n_seqs, s);
+    case 128: return launch_paged_attention_as<DT, 4>(a, n_seqs, s);
+    case 192: return launch_paged_attention_as<DT, 6>(a, n_seqs, s);
+    case 256: return launch_paged_attention_as<DT, 8>(a, n_seqs, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+RowArgs row_args(int n, int64_t row, int64_t head, const elmh_kv_pages& pages, const int32_t* table, int n_seqs,
+                 int max_pages, const int32_t* pos, const int32_t* seq, const elmh_rope* rope) {
+  const RowStrides st = row_strides(row, head, pages.n_kv, pages.head_dim);
+  RowArgs a{};
+  a.row = st.row;
+  a.head = st.head;
+  a.n = n;
+  a.pages = pages;
+  a.table = table;
+  a.n_seqs = n_seqs;
+  a.max_pages = max_pages;
+  a.pos = pos;
+  a.seq = seq;
+  if (rope) {
+    a.cs = rope->cos;
+    a.sn = rope->sin;
+    a.max_pos = rope->max_pos;
+    a.rot = rope->rot_dim;
+    a.inter = rope->interleaved;
+  }
+  return a;
+}
+dim3 row_grid(const RowArgs& a) {
+  const int64_t threads = (int64_t)a.n * a.pages.n_kv * row_lanes(a.pages.head_dim);
+  return dim3((unsigned)((threads + 255) / 256), 2);
+}
+
+}  // namespace
+
+hipError_t launch_rope_table(float* cs, float* sn, int64_t pos0, int64_t n, int rot_dim, double theta, const RopeBand& band,
+                             hipStream_t s) {
+  const int64_t blocks = (n * (rot_dim / 2) + 255) / 256;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  rope_table_kernel<<<(unsigned)blocks, 256, 0, s>>>(cs, sn, pos0, n, rot_dim / 2, theta, band);
+  return hipGetLastError();
+}
+
+hipError_t launch_rope(const float* x, float* y, int T, int n_heads, int hd, int64_t x_row, int64_t y_row,
+                       const elmh_rope& rope, const int32_t* pos, int64_t pos0, hipStream_t s) {
+  const int64_t pairs = (int64_t)T * n_heads * (hd / 2), width = (int64_t)n_heads * hd;
+  const int64_t blocks = (pairs + 255) / 256;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  rope_kernel<<<(unsigned)blocks, 256, 0, s>>>(x, y, pairs, n_heads, hd, x_row ? x_row : width, y_row ? y_row : width,
+                                               rope.cos, rope.sin, rope.max_pos, rope.rot_dim, rope.interleaved, pos, pos0);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_append(const float* k, const float* v, int n, int64_t row, int64_t head, const elmh_kv_pages& pages,
+                               const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq,
+                               const elmh_rope* rope, hipStream_t s) {
+  RowArgs a = row_args(n, row, head, pages, table, n_seqs, max_pages, pos, seq, rope);
+  a.k = k;
+  a.v = v;
+  paged_append_kernel<<<row_grid(a), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t head, const elmh_kv_pages& pages,
+                             const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq,
+                             hipStream_t s) {
+  RowArgs a = row_args(n, row, head, pages, table, n_seqs, max_pages, pos, seq, nullptr);
+  a.ko = k;
+  a.vo = v;
+  paged_read_kernel<<<row_grid(a), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+int paged_attention_parts(int n_seqs, int n_heads, int n_kv, int max_len) {
+  const int tiles = (n_heads / n_kv + kPaHeads - 1) / kPaHeads;
+  const int64_t rows = (int64_t)n_seqs * n_kv * tiles;
+  const int units = (max_len + kSplitUnit - 1) / kSplitUnit, most = (units + kPaLeastUnits - 1) / kPaLeastUnits;
+  const int64_t want = (2048 + rows - 1) / rows;
+  return (int)(want < most ? want : most);
+}
+
+size_t paged_attention_scratch_bytes(int n_seqs, int n_heads, int head_dim, int parts) {
+  return parts > 1 ? (size_t)n_seqs * n_heads * parts * (head_dim + 2) * sizeof(float) : 0;
+}
+
+hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int n_heads, const elmh_kv_pages& pages,
+                                  const int32_t* table, int n_seqs, int max_pages, const int32_t* lens, int max_len,
+                                  const elmh_rope* rope, int parts, float* scratch, hipStream_t s) {
+  PagedAttnArgs a{};
+  a.q = q;
+  a.out = out;
+  a.q_row = q_row ? q_row : (int64_t)n_heads * pages.head_dim;
+  a.n_heads = n_heads;
+  a.group = n_heads / pages.n_kv;
+  a.head_tiles = (a.group + kPaHeads - 1) / kPaHeads;
+  a.pages = pages;
+  a.table = table;
+  a.max_pages = max_pages;
+  a.lens = lens;
+  a.max_len = max_len;
+  if (rope) {
+    a.cs = rope->cos;
+    a.sn = rope->sin;
+    a.rot = rope->rot_dim;
+    a.inter = rope->interleaved;
+  }
+  a.parts = parts;
+  a.part_o = scratch;
+  a.part_s = scratch + (int64_t)n_seqs * n_heads * parts * pages.head_dim;
+  switch (pages.dtype) {
+    case ELMH_F32: return launch_paged_attention_of<ELMH_F32>(a, n_seqs, s);
+    case ELMH_F16: return launch_paged_attention_of<ELMH_F16>(a, n_seqs, s);
+    case ELMH_BF16: return launch_paged_attention_of<ELMH_BF16>(a, n_seqs, s);
+    case ELMH_Q8: return launch_paged_attention_of<ELMH_Q8>(a, n_seqs, s);
+    case ELMH_Q4: return launch_paged_attention_of<ELMH_Q4>(a, n_seqs, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace elmh

@@ -15,6 +15,9 @@ OK, ERR_ARG, ERR_HIP, ERR_NODEV, ERR_UNSUPPORTED, ERR_OOM = range(6)
 F32, Q8, Q4 = 0, 1, 2
 ACT_F32, ACT_INT8, ACT_INT8_TOKEN = 0, 1, 2
 EXACT, FAST = 0, 1
+F16, BF16 = 16, 17  # what else a paged cache holds
+KV_DTYPES = {"f32": F32, "f16": F16, "bf16": BF16, "q8": Q8, "q4": Q4}
+ROPE_LINEAR, ROPE_BANDS, ROPE_YARN = 1, 2, 3
 
 _lib = None
 
@@ -23,6 +26,26 @@ class ElmhError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"elmh error {code}: {msg}")
         self.code = code
+
+
+class KVPages(C.Structure):
+    """``elmh_kv_pages``: two pools of pages (device pointers, owned by the caller) and their scales."""
+    _fields_ = [("dtype", C.c_int), ("n_kv", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int64),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class Rope(C.Structure):
+    """``elmh_rope``: rotary tables [max_pos][rot_dim / 2] (device pointers) and how heads are rotated by them."""
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("max_pos", C.c_int), ("rot_dim", C.c_int), ("interleaved", C.c_int)]
+
+
+class RopeScaling(C.Structure):
+    """``elmh_rope_scaling``: frequencies of a context longer than orig_ctx."""
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("orig_ctx", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("magnitude", C.c_double)]
+
+    def __init__(self, kind, factor, orig_ctx=0.0, low=1.0, high=32.0, magnitude=1.0):
+        super().__init__(kind, factor, orig_ctx, low, high, magnitude)
 
 
 def lib():
@@ -42,6 +65,13 @@ def lib():
         L.elmh_weight_bytes.argtypes = [C.c_void_p]
         L.elmh_destroy.argtypes = [C.c_void_p]
         L.elmh_destroy.restype = None
+        v, i, l, d = C.c_void_p, C.c_int, C.c_int64, C.c_double
+        pages, rope, scaling = C.POINTER(KVPages), C.POINTER(Rope), C.POINTER(RopeScaling)
+        L.elmh_rope_table_dev.argtypes = [v, v, v, l, l, i, d, scaling]
+        L.elmh_rope_dev.argtypes = [v, v, v, i, i, i, l, l, rope, v, l]
+        L.elmh_paged_append_dev.argtypes = [v, v, v, i, l, l, pages, v, i, i, v, v, rope]
+        L.elmh_paged_read_dev.argtypes = [v, v, v, i, l, l, pages, v, i, i, v, v]
+        L.elmh_paged_attention_dev.argtypes = [v, v, v, l, i, pages, v, i, i, v, i, rope]
         _lib = L
     return _lib
 
@@ -63,6 +93,15 @@ def weight_layout(dtype, rows, cols):
     if rc:
         raise ElmhError(rc, lib().elmh_last_error(None).decode())
     return H.value, db.value, sb.value
+
+
+def kv_page_bytes(dtype, n_kv, head_dim, page_size):
+    """(bytes of one page's rows in one pool, bytes of its scales); pure host call, no GPU."""
+    data, scales = C.c_size_t(), C.c_size_t()
+    rc = lib().elmh_kv_page_bytes(C.c_int(dtype), C.c_int(n_kv), C.c_int(head_dim), C.c_int(page_size), C.byref(data), C.byref(scales))
+    if rc:
+        raise ElmhError(rc, lib().elmh_last_error(None).decode())
+    return data.value, scales.value
 
 
 def repack_host(dtype, rows, cols, data, scales):
@@ -312,6 +351,32 @@ class Context:
     def attention_matmul_fused(self):
         """True if the last attention_matmul_dev call had the attention kernel write the GEMM's operand."""
         return bool(lib().elmh_attention_matmul_fused(self.h))
+
+    # ---- many sequences over one paged key/value cache (device pointers; pages, rope and scaling: the structures above)
+    def rope_table_dev(self, cos_ptr, sin_ptr, pos0, n, rot_dim, theta, scaling=None):
+        """Rotary tables [n][rot_dim / 2] of positions pos0 .. pos0 + n - 1."""
+        self._check(lib().elmh_rope_table_dev(self.h, cos_ptr, sin_ptr, pos0, n, rot_dim, theta, scaling))
+
+    def rope_dev(self, x_ptr, y_ptr, T, n_heads, head_dim, rope, pos_ptr=None, pos0=0, x_row=0, y_row=0):
+        """y = x with each head rotated: row t at position pos[t], or pos0 + t."""
+        self._check(lib().elmh_rope_dev(self.h, x_ptr, y_ptr, T, n_heads, head_dim, x_row, y_row, rope, pos_ptr, pos0))
+
+    def paged_append_dev(self, k_ptr, v_ptr, n, pages, table_ptr, n_seqs, max_pages, pos_ptr, seq_ptr=None, rope=None, row=0,
+                         head=0):
+        """n tokens' keys (rotated with rope) and values into the cache at position pos[i] of sequence seq[i] (or i)."""
+        self._check(lib().elmh_paged_append_dev(self.h, k_ptr, v_ptr, n, row, head, pages, table_ptr, n_seqs, max_pages, pos_ptr,
+                                                seq_ptr, rope))
+
+    def paged_read_dev(self, k_ptr, v_ptr, n, pages, table_ptr, n_seqs, max_pages, pos_ptr, seq_ptr=None, row=0, head=0):
+        """The values that the cache holds of n positions, in f32."""
+        self._check(lib().elmh_paged_read_dev(self.h, k_ptr, v_ptr, n, row, head, pages, table_ptr, n_seqs, max_pages, pos_ptr,
+                                              seq_ptr))
+
+    def paged_attention_dev(self, q_ptr, out_ptr, n_heads, pages, table_ptr, n_seqs, max_pages, lens_ptr, max_len, rope=None,
+                            q_row=0):
+        """Attention of one new token a sequence over its first lens[s] <= max_len positions in the cache."""
+        self._check(lib().elmh_paged_attention_dev(self.h, q_ptr, out_ptr, q_row, n_heads, pages, table_ptr, n_seqs, max_pages,
+                                                   lens_ptr, max_len, rope))
 
     def argmax_dev(self, x_ptr, rows, n, out_ptr):
         self._check(lib().elmh_argmax_dev(self.h, C.c_void_p(x_ptr), C.c_int(rows), C.c_int64(n), C.c_void_p(out_ptr)))

@@ -46,6 +46,9 @@ typedef enum {
 /* weight dtypes: the values of edgelm's DType (include/edgelm/graph.hpp:17) */
 enum { ELMH_F32 = 0, ELMH_Q8 = 1, ELMH_Q4 = 2 };
 
+/* what else a paged cache holds (16-bit floats; edgelm has no such types) */
+enum { ELMH_F16 = 16, ELMH_BF16 = 17 };
+
 /* activation handling */
 enum {
   ELMH_ACT_F32 = 0,        /* Session act_quant = false (runtime.hpp:25) */
@@ -241,6 +244,83 @@ int elmh_argmax_dev(elmh_ctx* ctx, const float* x, int rows, int64_t n, int32_t*
  * one context run in stream order (they share a small counter in the context). */
 int elmh_argmax_step_dev(elmh_ctx* ctx, const float* x, int64_t n, int32_t* out, int32_t* pos_dev, int32_t* ring,
                          int ring_len);
+
+/* ---- many sequences over one paged key/value cache (device pointers, asynchronous on the context stream) ----
+ * No counterpart in edgelm, whose KVLayer (kernels.hpp:22) is one f32 cache of max_ctx positions per Session: these serve a
+ * batch of sequences of different lengths that share two pools of pages, with smaller cache types and longer contexts.
+ *
+ * The pools. Keys and values are rows of head_dim values at [page][kv head][slot], page_size slots a page (a multiple of 16):
+ *   ELMH_F32, ELMH_F16, ELMH_BF16   the values (16-bit: rounded to nearest even as they are written);
+ *   ELMH_Q8   int8, one f32 scale per row at [page][kv head][slot]: the row's largest magnitude / 127, levels to the nearest,
+ *             halves away from zero (edgelm's quantize_q8 of a weight row, model.cpp:150-163);
+ *   ELMH_Q4   levels -8 .. 7 held as 0 .. 15, one f32 scale per 32 values at [page][kv head][group][slot]: the group's first value
+ *             of largest magnitude / -8 (edgelm's quantize_q4, model.cpp:165-190). A byte holds two neighbouring values, the
+ *             first in the low nibble; a key row's bytes are [c][j][b], values 32 j + 8 c + 2 b; a value row's [i][j],
+ *             values 32 j + 2 i.
+ * Keys are stored rotated. head_dim is 32, 64, 96, 128, 192 or 256. The caller owns pools and scales (each on 16 bytes; scales
+ * are NULL for the float types) and the page table [n_seqs][max_pages]: position p of sequence s is slot p % page_size of page
+ * table[s][p / page_size]. Entries outside 0 .. n_pages - 1 name no page: nothing is read or written through them. One page may
+ * be in several sequences (a shared prefix); a position is written at most once a call (written twice, its row is
+ * unspecified). */
+typedef struct {
+  int dtype, n_kv, head_dim, page_size;
+  int64_t n_pages;
+  void *k, *v;
+  float *k_scale, *v_scale;
+} elmh_kv_pages;
+/* Bytes of one page's rows in one pool, and of its scales (0 for the float types). Pure host call. */
+int elmh_kv_page_bytes(int dtype, int n_kv, int head_dim, int page_size, size_t* data, size_t* scales);
+
+/* Rotary positions: tables cos and sin [max_pos][rot_dim / 2] (edgelm's RopeTable, kernels_ref.cpp:11-21, has rot_dim =
+ * head_dim). The first rot_dim values of a head are rotated, the others pass: pairs (i, i + rot_dim / 2), or with interleaved
+ * (2 i, 2 i + 1); (a, b) becomes (a cos - b sin, b cos + a sin), each product and sum rounded to f32 by itself. */
+typedef struct {
+  const float *cos, *sin;
+  int max_pos, rot_dim, interleaved;
+} elmh_rope;
+/* Frequencies f of a longer context than the model's own orig_ctx:
+ *   ELMH_ROPE_LINEAR  f / factor;
+ *   ELMH_ROPE_BANDS   by the turns t = orig_ctx f / 2 pi a pair makes over orig_ctx: kept above `high`, f / factor below `low`,
+ *                     blended linearly in t between;
+ *   ELMH_ROPE_YARN    by the pair's index, blended linearly between the pairs (rounded outwards) that make `high` and `low` turns.
+ * Both tables are multiplied by magnitude (1, or what the model's attention was scaled by). */
+enum { ELMH_ROPE_LINEAR = 1, ELMH_ROPE_BANDS = 2, ELMH_ROPE_YARN = 3 };
+typedef struct {
+  int kind;
+  double factor, orig_ctx, low, high, magnitude;
+} elmh_rope_scaling;
+/* cos and sin [n][rot_dim / 2] of positions pos0 .. pos0 + n - 1: the angle p theta^(-2 i / rot_dim), scaled unless scaling is
+ * NULL, taken in f64 and each value rounded to f32 once. */
+int elmh_rope_table_dev(elmh_ctx* ctx, float* cos, float* sin, int64_t pos0, int64_t n, int rot_dim, double theta,
+                        const elmh_rope_scaling* scaling);
+/* y = x with each head rotated: rows of n_heads * head_dim values, x_row and y_row apart (0: contiguous), row t at position
+ * pos[t] (device), or pos0 + t where pos is NULL. A row whose position is outside the tables is left as it was. y may be x
+ * (with one stride); otherwise they do not overlap. head_dim: even, up to 1024. */
+int elmh_rope_dev(elmh_ctx* ctx, const float* x, float* y, int T, int n_heads, int head_dim, int64_t x_row, int64_t y_row,
+                  const elmh_rope* rope, const int32_t* pos, int64_t pos0);
+/* Writes n tokens' keys (rotated first unless rope is NULL) and values into the cache: row i's head h at k + i * row + h *
+ * head, strides in values (0: contiguous [n][n_kv][head_dim]), goes to position pos[i] of sequence seq[i] (i where seq is
+ * NULL, and then n <= n_seqs). A row is skipped, and the cache left as it was, where its position is negative (padding), past
+ * the table's pages or the rotary tables, its sequence is not one of n_seqs, or the table names no page. Finite values. */
+int elmh_paged_append_dev(elmh_ctx* ctx, const float* k, const float* v, int n, int64_t row, int64_t head,
+                          const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages, const int32_t* pos,
+                          const int32_t* seq, const elmh_rope* rope);
+/* The reverse: the values that the cache holds (level * scale, in f32) of n positions, keys as stored (rotated). Skipped rows
+ * are left as they were. With row = head_dim and head = n * head_dim the rows form a contiguous cache
+ * [n_kv][n][head_dim] as elmh_attention_dev keeps it. */
+int elmh_paged_read_dev(elmh_ctx* ctx, float* k, float* v, int n, int64_t row, int64_t head, const elmh_kv_pages* pages,
+                        const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq);
+/* Attention of one new token a sequence: out[s, h] = softmax over positions p < lens[s] of (q . k_p) / sqrt(head_dim), applied
+ * to v_p, query head h reading kv head h / (n_heads / n_kv). q's rows are q_row values apart (0: contiguous) and, with rope,
+ * rotated at position lens[s] - 1: the new token's key and value are in the cache already (elmh_paged_append_dev). out [n_seqs,
+ * n_heads * head_dim], not overlapping q. lens is read on the device and bounded to 0 .. max_len; max_len, the host's bound,
+ * sizes the launch. A sequence of length 0 (padding) gives zeros; positions of no page are left out; slots behind a sequence's
+ * end may hold anything. Products and sums in f32 or as exact as it (quantized levels are multiplied as they are).
+ * Long sequences are split over workgroups and joined, in a device buffer the context allocates and grows outside capture
+ * (elmh_scratch_generation); results do not depend on the order in which the parts end. */
+int elmh_paged_attention_dev(elmh_ctx* ctx, const float* q, float* out, int64_t q_row, int n_heads,
+                             const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages,
+                             const int32_t* lens, int max_len, const elmh_rope* rope);
 
 /* ---- test hooks ----
  * quantize_act_row on the device (host pointers; q [T,K], d [T,K/32]). */
