@@ -4,6 +4,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "elm_dpp.h"
 #include "elm_paged.h"
 #include "elm_quant.h"
@@ -21,15 +23,75 @@ using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 // ---------------------------------------------------------------- rotary tables and rotation
 
+// sin and cos of a in f64, to some 2^-44: a less its nearest multiple of pi / 2 (in two parts, so that nothing is lost up to 2^31
+// turns), then the Taylor sums to r^13 and r^14 on [-pi/4, pi/4] (the first terms left out are under 2^-45). The result is
+// rounded to f32, which needs no more; a library sine in f64 costs three times the instructions.
+__device__ __forceinline__ void sincos_f64(double a, double& sn, double& cs) {
+  const double k = rint(a * 0.63661977236758134308);
+  double r = fma(k, -1.57079632679489655800, a);
+  r = fma(k, -6.12323399573676603587e-17, r);
+  const double z = r * r;
+  double s = fma(z, 1.0 / 6227020800, -1.0 / 39916800);
+  s = fma(s, z, 1.0 / 362880);
+  s = fma(s, z, -1.0 / 5040);
+  s = fma(s, z, 1.0 / 120);
+  s = fma(s, z, -1.0 / 6);
+  s = fma(s * z, r, r);
+  double c = fma(z, -1.0 / 87178291200, 1.0 / 479001600);
+  c = fma(c, z, -1.0 / 3628800);
+  c = fma(c, z, 1.0 / 40320);
+  c = fma(c, z, -1.0 / 720);
+  c = fma(c, z, 1.0 / 24);
+  c = fma(c, z, -0.5);
+  c = fma(c, z, 1.0);
+  const int q = (int)k;  // a position under 2^31 at a frequency of at most 1: |k| < 2^31
+  const bool swap = q & 1;
+  const double u = swap ? c : s, v = swap ? s : c;
+  sn = q & 2 ? -u : u;
+  cs = (q + 1) & 2 ? -v : v;
+}
+
+// Workgroups of whole rows (positions): each takes the pairs' frequencies into LDS once (a power in f64 costs as much as many
+// angles), then its threads W neighbouring pairs at a time. Bound by the tables' writes.
+template <int W>
 __global__ __launch_bounds__(256) void rope_table_kernel(float* __restrict__ cs, float* __restrict__ sn, int64_t pos0,
-                                                         int64_t n, int half, double theta, RopeBand band) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= n * half) return;
-  const int i = (int)(at % half);
-  const double f = rope_scaled(band, pow(theta, -2.0 * i / (2 * half)), i);
-  const double a = (double)(pos0 + at / half) * f;
-  cs[at] = (float)(cos(a) * band.magnitude);
-  sn[at] = (float)(sin(a) * band.magnitude);
+                                                         int64_t n, int half, int rows, double theta, RopeBand band) {
+  __shared__ double freq[512];
+  for (int i = threadIdx.x; i < half; i += 256) freq[i] = rope_scaled(band, pow(theta, -2.0 * i / (2 * half)), i);
+  __syncthreads();
+  const int per = half / W;
+  const int64_t first = (int64_t)blockIdx.x * rows;
+  const int here = (int)(n - first < rows ? n - first : rows);
+  const int drow = 256 / per, dcol = 256 % per;
+  int row = threadIdx.x / per, col = threadIdx.x % per;
+  while (row < here) {
+    const double p = (double)(pos0 + first + row);
+    float c[W], s[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      double u, v;
+      sincos_f64(p * freq[W * col + w], u, v);
+      s[w] = (float)(u * band.magnitude);
+      c[w] = (float)(v * band.magnitude);
+    }
+    const int64_t at = (first + row) * half + W * col;
+    if constexpr (W == 4) {
+      *reinterpret_cast<f32x4*>(cs + at) = f32x4{c[0], c[1], c[2], c[3]};
+      *reinterpret_cast<f32x4*>(sn + at) = f32x4{s[0], s[1], s[2], s[3]};
+    } else {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        cs[at + w] = c[w];
+        sn[at + w] = s[w];
+      }
+    }
+    row += drow;
+    col += dcol;
+    if (col >= per) {
+      col -= per;
+      ++row;
+    }
+  }
 }
 
 // One thread a pair: (i, i + rot / 2) or (2 i, 2 i + 1), and past the rotated part two neighbours that pass.
@@ -792,9 +854,17 @@ dim3 row_grid(const RowArgs& a) {
 
 hipError_t launch_rope_table(float* cs, float* sn, int64_t pos0, int64_t n, int rot_dim, double theta, const RopeBand& band,
                              hipStream_t s) {
-  const int64_t blocks = (n * (rot_dim / 2) + 255) / 256;
+  const int half = rot_dim / 2;
+  const bool wide = half % 4 == 0 && aligned16(cs) && aligned16(sn);
+  // rows a workgroup: up to 16 passes of its threads, as long as some 2048 workgroups are left
+  const int64_t one = std::max<int64_t>(1, 256 / (wide ? half / 4 : half));
+  const int64_t rows = one * std::min<int64_t>(16, std::max<int64_t>(1, n / (one * 2048)));
+  const int64_t blocks = (n + rows - 1) / rows;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  rope_table_kernel<<<(unsigned)blocks, 256, 0, s>>>(cs, sn, pos0, n, rot_dim / 2, theta, band);
+  if (wide)
+    rope_table_kernel<4><<<(unsigned)blocks, 256, 0, s>>>(cs, sn, pos0, n, half, (int)rows, theta, band);
+  else
+    rope_table_kernel<1><<<(unsigned)blocks, 256, 0, s>>>(cs, sn, pos0, n, half, (int)rows, theta, band);
   return hipGetLastError();
 }
 
