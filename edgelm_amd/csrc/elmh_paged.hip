@@ -94,29 +94,97 @@ __global__ __launch_bounds__(256) void rope_table_kernel(float* __restrict__ cs,
   }
 }
 
-// One thread a pair: (i, i + rot / 2) or (2 i, 2 i + 1), and past the rotated part two neighbours that pass.
-__global__ __launch_bounds__(256) void rope_kernel(const float* x, float* y, int64_t pairs, int n_heads, int hd,
-                                                   int64_t x_row, int64_t y_row, const float* __restrict__ cs,
-                                                   const float* __restrict__ sn, int max_pos, int rot, int inter,
-                                                   const int32_t* __restrict__ pos, int64_t pos0) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= pairs) return;
-  const int i = (int)(at % (hd / 2)), half = rot / 2;
-  const int64_t row = at / (hd / 2), t = row / n_heads;
-  const int64_t p = pos ? pos[t] : pos0 + t;
-  if (p < 0 || p >= max_pos) return;
-  const int64_t head = (row % n_heads) * hd;
-  const bool turned = i < half;
-  const int a = turned && !inter ? i : 2 * i, b = turned && !inter ? i + half : 2 * i + 1;
-  float u = x[t * x_row + head + a], v = x[t * x_row + head + b];
-  if (turned) {
-    const float c = cs[p * half + i], s = sn[p * half + i];
-    const float u0 = u;
-    u = u0 * c - v * s;
-    v = v * c + u0 * s;
+// What a thread does is the same for every row: it finds its head and values once and then takes rows blockIdx.y, + gridDim.y,
+// ..., kRopeRows at a time. Both of a pair are one thread's, so that rows may be rotated in place. Bound by reading and writing
+// the rows.
+constexpr int kRopeRows = 4;
+
+// Where everything is aligned: per head rot / 8 threads with two groups of four values, i .. and i + rot / 2 .. (half layout),
+// and (hd - rot) / 4 with four that pass; interleaved: hd / 4 threads with four neighbours. A wave's accesses are contiguous.
+__global__ __launch_bounds__(256) void rope_quads_kernel(const float* x, float* y, int T, int per_head, int n_heads, int hd,
+                                                         int64_t x_row, int64_t y_row, const float* __restrict__ cs,
+                                                         const float* __restrict__ sn, int max_pos, int rot, int inter,
+                                                         const int32_t* __restrict__ pos, int64_t pos0) {
+  const int u = blockIdx.x * 256 + threadIdx.x, head = u / per_head, i = u % per_head, half = rot / 2;
+  if (head >= n_heads) return;
+  const bool split = !inter && i < rot / 8, near = inter && i < rot / 4, turned = split || near;
+  if (!turned && x == y) return;
+  const int a = head * hd + 4 * i + (turned || inter ? 0 : half);  // half layout: the passing values follow both halves
+  const int at = near ? 2 * i : 4 * i;
+  for (int t0 = blockIdx.y * kRopeRows; t0 < T; t0 += gridDim.y * kRopeRows) {
+    f32x4 va[kRopeRows], vb[kRopeRows], c[kRopeRows], s[kRopeRows];
+    bool live[kRopeRows];
+#pragma unroll
+    for (int r = 0; r < kRopeRows; ++r) {
+      const int t = min(t0 + r, T - 1);
+      const int64_t p = pos ? pos[t] : pos0 + t;
+      live[r] = t0 + r < T && p >= 0 && p < max_pos;
+      const float* src = x + t * x_row + a;
+      const int64_t row = (live[r] ? p : 0) * half;
+      va[r] = *reinterpret_cast<const f32x4*>(src);
+      if (split) {
+        vb[r] = *reinterpret_cast<const f32x4*>(src + half);
+        c[r] = *reinterpret_cast<const f32x4*>(cs + row + at);
+        s[r] = *reinterpret_cast<const f32x4*>(sn + row + at);
+      } else if (near) {
+        const float2 c2 = *reinterpret_cast<const float2*>(cs + row + at), s2 = *reinterpret_cast<const float2*>(sn + row + at);
+        c[r] = f32x4{c2.x, c2.x, c2.y, c2.y};
+        s[r] = f32x4{-s2.x, s2.x, -s2.y, s2.y};  // u c - v s = u c + v (-s), to the bit
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRopeRows; ++r) {
+      if (!live[r]) continue;
+      float* dst = y + (int64_t)(t0 + r) * y_row + a;
+      f32x4 o = va[r];
+      if (split) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = va[r][e] * c[r][e] - vb[r][e] * s[r][e];
+        f32x4 q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = vb[r][e] * c[r][e] + va[r][e] * s[r][e];
+        *reinterpret_cast<f32x4*>(dst + half) = q;
+      } else if (near) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = va[r][e] * c[r][e] + va[r][e ^ 1] * s[r][e];
+      }
+      *reinterpret_cast<f32x4*>(dst) = o;
+    }
   }
-  y[t * y_row + head + a] = u;
-  y[t * y_row + head + b] = v;
+}
+
+// Any alignment: hd / 2 threads a head, each a pair, or two neighbours that pass
+__global__ __launch_bounds__(256) void rope_pairs_kernel(const float* x, float* y, int T, int per_head, int n_heads, int hd,
+                                                         int64_t x_row, int64_t y_row, const float* __restrict__ cs,
+                                                         const float* __restrict__ sn, int max_pos, int rot, int inter,
+                                                         const int32_t* __restrict__ pos, int64_t pos0) {
+  const int u = blockIdx.x * 256 + threadIdx.x, head = u / per_head, i = u % per_head, half = rot / 2;
+  if (head >= n_heads) return;
+  const bool turned = i < half, split = turned && !inter;
+  if (!turned && x == y) return;
+  const int a = head * hd + (split ? i : 2 * i), b = split ? a + half : a + 1;
+  for (int t0 = blockIdx.y * kRopeRows; t0 < T; t0 += gridDim.y * kRopeRows) {
+    float va[kRopeRows], vb[kRopeRows], c[kRopeRows], s[kRopeRows];
+    bool live[kRopeRows];
+#pragma unroll
+    for (int r = 0; r < kRopeRows; ++r) {
+      const int t = min(t0 + r, T - 1);
+      const int64_t p = pos ? pos[t] : pos0 + t;
+      live[r] = t0 + r < T && p >= 0 && p < max_pos;
+      const int64_t at = (live[r] ? p : 0) * half + (turned ? i : 0);
+      va[r] = x[t * x_row + a];
+      vb[r] = x[t * x_row + b];
+      c[r] = cs[at];
+      s[r] = sn[at];
+    }
+#pragma unroll
+    for (int r = 0; r < kRopeRows; ++r) {
+      if (!live[r]) continue;
+      float* dst = y + (int64_t)(t0 + r) * y_row;
+      dst[a] = turned ? va[r] * c[r] - vb[r] * s[r] : va[r];
+      dst[b] = turned ? vb[r] * c[r] + va[r] * s[r] : vb[r];
+    }
+  }
 }
 
 // ---------------------------------------------------------------- rows into pages and back
@@ -156,119 +224,209 @@ __device__ __forceinline__ float rotated(const float* x, int d, const float* cs,
   return second ? self * c + other * s : self * c - other * s;
 }
 
-// Lanes that share a row, eight values each: head_dim / 8 rounded up to a power of two (the rest idle)
-ELM_HD int row_lanes(int hd) { return hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
+// Rows go by eight lanes each: lane c of them holds values 32 j + 4 c .. + 3 of every 32-value group j, so that eight lanes read
+// or write 128 contiguous bytes of f32 a group, the group's q4 scale is a matter of eight lanes, and its eight 4-bit levels
+// lie in neighbouring bytes. A workgroup: 32 rows of one kv head in one pool (grid: rows, heads, pools).
+constexpr int kRowLanes = 8;
+constexpr int kRowsPerBlock = 256 / kRowLanes;
 
-__global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
-  const elmh_kv_pages& pg = a.pages;
-  const int hd = pg.head_dim, lanes = row_lanes(hd);
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
-  const int c = threadIdx.x % lanes, d0 = 8 * c;
-  const bool keys = blockIdx.y == 0, in = at < (int64_t)a.n * pg.n_kv && d0 < hd;
-  const int t = (int)(at / pg.n_kv), h = (int)(at % pg.n_kv);
-  RowPlace w{-1, 0, 0};
-  if (in) w = row_place(a, t);
-  const bool live = w.page >= 0;
-  float x[8];
+// max over a row's eight lanes, in one instruction a step
+__device__ __forceinline__ float row_max8(float v) {
+  v = fmaxf(v, dpp_f<kDppQuadXor1>(v));
+  v = fmaxf(v, dpp_f<kDppQuadXor2>(v));
+  return fmaxf(v, dpp_f<kDppHalfMirror>(v));
+}
+
+// x: 4 * NB values of lane c, NB groups. VEC: 16-byte loads (the host has checked that every one is aligned, and that a lane's
+// four values are either all rotated or none, with their partners four values too).
+template <int NB, bool VEC>
+__device__ __forceinline__ void load_row(float (&x)[NB][4], const float* src, int c, const float* cs, const float* sn, int half,
+                                         int inter) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.f;
-  if (live) {
-    const float* src = (keys ? a.k : a.v) + t * a.row + h * a.head;
-    const int half = a.rot / 2;
+  for (int j = 0; j < NB; ++j) {
+    const int d = 32 * j + 4 * c;
+    if constexpr (VEC) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(src + d);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      x[e] = keys && a.cs ? rotated(src, d0 + e, a.cs + (int64_t)w.pos * half, a.sn + (int64_t)w.pos * half, half, a.inter)
-                          : src[d0 + e];
-  }
-  const int64_t row = live ? kv_row(w.page, h, w.slot, pg.n_kv, pg.page_size) : 0;
-  void* pool = keys ? pg.k : pg.v;
-  float* scales = keys ? pg.k_scale : pg.v_scale;
-  if (pg.dtype == ELMH_Q8) {
-    float amax = 0.f;
+      for (int e = 0; e < 4; ++e) x[j][e] = v[e];
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-    for (int off = lanes / 2; off; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
-    const float s = amax / 127.f;
-    int q[8];
-    elm_q8_group<8>(x, s == 0.f ? 1.f : s, q);
-    if (!live) return;
-    u32x2 b{0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) b[e / 4] |= (uint32_t)(q[e] & 0xFF) << (8 * (e % 4));
-    *reinterpret_cast<u32x2*>(static_cast<int8_t*>(pool) + row * hd + d0) = b;
-    if (c == 0) scales[row] = s;
-    return;
-  }
-  if (pg.dtype == ELMH_Q4) {
-    // the group's first value of largest magnitude: in this lane, then over the four lanes of the group
-    float m = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) m = fabsf(x[e]) > fabsf(m) ? x[e] : m;
-#pragma unroll
-    for (int off = 1; off <= 2; off <<= 1) {
-      const float o = __shfl_xor(m, off, 64);
-      const bool lower = c & off;  // the other lane's values come first
-      m = lower ? (fabsf(o) >= fabsf(m) ? o : m) : (fabsf(o) > fabsf(m) ? o : m);
+      for (int e = 0; e < 4; ++e) x[j][e] = cs ? rotated(src, d + e, cs, sn, half, inter) : src[d + e];
     }
-    const float s = m / -8.f, div = s == 0.f ? 1.f : s;
-    if (!live) return;
-    uint32_t nib[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float r = x[e] / div;
-      nib[e] = (uint32_t)((int)fminf(7.f, fmaxf(-8.f, copysignf(floorf(fabsf(r) + 0.5f), r))) + 8);
-    }
-    uint8_t* dst = static_cast<uint8_t*>(pool) + row * (hd / 2);
-#pragma unroll
-    for (int e = 0; e < 8; e += 2)
-      dst[keys ? q4_key_byte(d0 + e, hd) : q4_value_byte(d0 + e, hd)] = (uint8_t)(nib[e] | nib[e + 1] << 4);
-    if (c % 4 == 0) scales[kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, hd / 32) + (int64_t)(c / 4) * pg.page_size] = s;
-    return;
   }
-  if (!live) return;
+  if constexpr (VEC) {
+    if (!cs) return;
+    // the partners of the half layout are another lane's, or this one's of another group: read again (they are in L1)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if (pg.dtype == ELMH_F32)
-      static_cast<float*>(pool)[row * hd + d0 + e] = x[e];
-    else if (pg.dtype == ELMH_F16)
-      static_cast<_Float16*>(pool)[row * hd + d0 + e] = (_Float16)x[e];
-    else
-      static_cast<__bf16*>(pool)[row * hd + d0 + e] = (__bf16)x[e];
+    for (int j = 0; j < NB; ++j) {
+      const int d = 32 * j + 4 * c;
+      if (d >= 2 * half) continue;
+      if (inter) {
+        const u32x2 co = *reinterpret_cast<const u32x2*>(cs + d / 2), si = *reinterpret_cast<const u32x2*>(sn + d / 2);
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const float cc = __uint_as_float(co[e / 2]), ss = __uint_as_float(si[e / 2]), u = x[j][e], v = x[j][e + 1];
+          x[j][e] = u * cc - v * ss;
+          x[j][e + 1] = v * cc + u * ss;
+        }
+      } else {
+        const bool second = d >= half;
+        const int i = second ? d - half : d;
+        const f32x4 o = *reinterpret_cast<const f32x4*>(src + (second ? i : d + half));
+        const f32x4 co = *reinterpret_cast<const f32x4*>(cs + i), si = *reinterpret_cast<const f32x4*>(sn + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ss = second ? si[e] : -si[e];  // u c - v s = u c + v (-s), to the bit
+          x[j][e] = x[j][e] * co[e] + o[e] * ss;
+        }
+      }
+    }
   }
 }
 
-__global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a) {
+template <int DT, int NB, bool VEC>
+__global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
+  constexpr int HD = 32 * NB;
   const elmh_kv_pages& pg = a.pages;
-  const int hd = pg.head_dim, lanes = row_lanes(hd);
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
-  const int c = threadIdx.x % lanes, d0 = 8 * c;
-  if (at >= (int64_t)a.n * pg.n_kv || d0 >= hd) return;
-  const bool keys = blockIdx.y == 0;
-  const int t = (int)(at / pg.n_kv), h = (int)(at % pg.n_kv);
+  const int t = blockIdx.x * kRowsPerBlock + threadIdx.x / kRowLanes, c = threadIdx.x % kRowLanes, h = blockIdx.y;
+  const bool keys = blockIdx.z == 0;
+  if (t >= a.n) return;  // whole rows: the lanes of a row stay together
+  const RowPlace w = row_place(a, t);
+  if (w.page < 0) return;
+  const bool turn = keys && a.cs;
+  const int half = a.rot / 2;
+  const int64_t at = (int64_t)w.pos * half;
+  float x[NB][4];
+  load_row<NB, VEC>(x, (keys ? a.k : a.v) + t * a.row + h * a.head, c, turn ? a.cs + at : nullptr, turn ? a.sn + at : nullptr,
+                    half, a.inter);
+  const int64_t row = kv_row(w.page, h, w.slot, pg.n_kv, pg.page_size);
+  uint8_t* dst = static_cast<uint8_t*>(keys ? pg.k : pg.v) + row * (DT == ELMH_F32 ? 4 * HD : DT == ELMH_Q8 ? HD : DT == ELMH_Q4 ? HD / 2 : 2 * HD);
+  float* scales = keys ? pg.k_scale : pg.v_scale;
+  if constexpr (DT == ELMH_F32) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) *reinterpret_cast<f32x4*>(dst + 128 * j + 16 * c) = f32x4{x[j][0], x[j][1], x[j][2], x[j][3]};
+  } else if constexpr (DT == ELMH_F16 || DT == ELMH_BF16) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (DT == ELMH_F16) u[e] = __builtin_bit_cast(uint16_t, (_Float16)x[j][e]);
+        else u[e] = __builtin_bit_cast(uint16_t, (__bf16)x[j][e]);
+      }
+      *reinterpret_cast<u32x2*>(dst + 64 * j + 8 * c) = u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+    }
+  } else if constexpr (DT == ELMH_Q8) {
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(x[j][e]));
+    amax = row_max8(amax);
+    const float s = amax / 127.f, div = s == 0.f ? 1.f : s;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      int q[4];
+      elm_q8_group<4>(x[j], div, q);
+      *reinterpret_cast<uint32_t*>(dst + 32 * j + 4 * c) =
+          (q[0] & 0xFF) | (q[1] & 0xFF) << 8 | (q[2] & 0xFF) << 16 | (uint32_t)(q[3] & 0xFF) << 24;
+    }
+    if (c == 0) scales[row] = s;
+  } else {
+    uint32_t b[NB];  // a group's two bytes of this lane
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      // the first value of largest magnitude: of this lane's four, then of the eight lanes (a tie is the lower lane's)
+      float m = x[j][0];
+#pragma unroll
+      for (int e = 1; e < 4; ++e) m = fabsf(x[j][e]) > fabsf(m) ? x[j][e] : m;
+      const float amax = row_max8(fabsf(m));
+      const uint32_t have = (uint32_t)(__ballot(fabsf(m) == amax) >> (threadIdx.x & 56)) & 0xFFu;
+      // no lane has it only if a value is not a number
+      const float s = __shfl(m, (threadIdx.x & 56) + (have ? __builtin_ctz(have) : 0), 64) / -8.f, div = s == 0.f ? 1.f : s;
+      uint32_t nib[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float r = x[j][e] / div;
+        nib[e] = (uint32_t)((int)fminf(7.f, fmaxf(-8.f, copysignf(floorf(fabsf(r) + 0.5f), r))) + 8);
+      }
+      b[j] = nib[0] | nib[1] << 4 | nib[2] << 8 | nib[3] << 12;
+      if (c == 0) scales[kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, NB) + (int64_t)j * pg.page_size] = s;
+    }
+    if (keys) {  // [c / 2][j]: words of which this lane has one half
+#pragma unroll
+      for (int j = 0; j < NB; ++j) *reinterpret_cast<uint16_t*>(dst + (c / 2) * 4 * NB + 4 * j + 2 * (c % 2)) = (uint16_t)b[j];
+    } else {  // [2 c][j], [2 c + 1][j]: all of this lane's bytes are neighbours
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        dst[2 * c * NB + j] = (uint8_t)b[j];
+        dst[(2 * c + 1) * NB + j] = (uint8_t)(b[j] >> 8);
+      }
+    }
+  }
+}
+
+template <int DT, int NB, bool VEC>
+__global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a) {
+  constexpr int HD = 32 * NB;
+  const elmh_kv_pages& pg = a.pages;
+  const int t = blockIdx.x * kRowsPerBlock + threadIdx.x / kRowLanes, c = threadIdx.x % kRowLanes, h = blockIdx.y;
+  const bool keys = blockIdx.z == 0;
+  if (t >= a.n) return;
   const RowPlace w = row_place(a, t);
   if (w.page < 0) return;
   const int64_t row = kv_row(w.page, h, w.slot, pg.n_kv, pg.page_size);
-  const void* pool = keys ? pg.k : pg.v;
+  const uint8_t* src = static_cast<const uint8_t*>(keys ? pg.k : pg.v) +
+                       row * (DT == ELMH_F32 ? 4 * HD : DT == ELMH_Q8 ? HD : DT == ELMH_Q4 ? HD / 2 : 2 * HD);
   const float* scales = keys ? pg.k_scale : pg.v_scale;
-  float* dst = (keys ? a.ko : a.vo) + t * a.row + h * a.head + d0;
+  float x[NB][4];
+  if constexpr (DT == ELMH_F32) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float x;
-    if (pg.dtype == ELMH_F32) {
-      x = static_cast<const float*>(pool)[row * hd + d0 + e];
-    } else if (pg.dtype == ELMH_F16) {
-      x = (float)static_cast<const _Float16*>(pool)[row * hd + d0 + e];
-    } else if (pg.dtype == ELMH_BF16) {
-      x = (float)static_cast<const __bf16*>(pool)[row * hd + d0 + e];
-    } else if (pg.dtype == ELMH_Q8) {
-      x = (float)static_cast<const int8_t*>(pool)[row * hd + d0 + e] * scales[row];
-    } else {
-      const int d = d0 + e;
-      const int b = static_cast<const uint8_t*>(pool)[row * (hd / 2) + (keys ? q4_key_byte(d & ~1, hd) : q4_value_byte(d & ~1, hd))];
-      x = (float)((d & 1 ? b >> 4 : b & 15) - 8) *
-          scales[kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, hd / 32) + (int64_t)(d / 32) * pg.page_size];
+    for (int j = 0; j < NB; ++j) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(src + 128 * j + 16 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = v[e];
     }
-    dst[e] = x;
+  } else if constexpr (DT == ELMH_F16 || DT == ELMH_BF16) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const u32x2 u = *reinterpret_cast<const u32x2*>(src + 64 * j + 8 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint16_t b = (uint16_t)(u[e / 2] >> (16 * (e % 2)));
+        if constexpr (DT == ELMH_F16) x[j][e] = (float)__builtin_bit_cast(_Float16, b);
+        else x[j][e] = __uint_as_float((uint32_t)b << 16);
+      }
+    }
+  } else if constexpr (DT == ELMH_Q8) {
+    const float s = scales[row];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(src + 32 * j + 4 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = (float)(int8_t)(u >> (8 * e)) * s;
+    }
+  } else {
+    const float* sc = scales + kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, NB);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const uint32_t u = keys ? *reinterpret_cast<const uint16_t*>(src + (c / 2) * 4 * NB + 4 * j + 2 * (c % 2))
+                              : src[2 * c * NB + j] | (uint32_t)src[(2 * c + 1) * NB + j] << 8;
+      const float s = sc[(int64_t)j * pg.page_size];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = (float)((int)(u >> (4 * e) & 15) - 8) * s;
+    }
+  }
+  float* dst = (keys ? a.ko : a.vo) + t * a.row + h * a.head;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int d = 32 * j + 4 * c;
+    if constexpr (VEC) {
+      *reinterpret_cast<f32x4*>(dst + d) = f32x4{x[j][0], x[j][1], x[j][2], x[j][3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[d + e] = x[j][e];
+    }
   }
 }
 
@@ -845,9 +1003,41 @@ RowArgs row_args(int n, int64_t row, int64_t head, const elmh_kv_pages& pages, c
   }
   return a;
 }
-dim3 row_grid(const RowArgs& a) {
-  const int64_t threads = (int64_t)a.n * a.pages.n_kv * row_lanes(a.pages.head_dim);
-  return dim3((unsigned)((threads + 255) / 256), 2);
+template <int DT, int NB>
+void launch_rows_as(const RowArgs& a, bool vec, hipStream_t s) {
+  const dim3 grid((a.n + kRowsPerBlock - 1) / kRowsPerBlock, a.pages.n_kv, 2);
+  if (a.ko) {
+    if (vec) paged_read_kernel<DT, NB, true><<<grid, 256, 0, s>>>(a);
+    else paged_read_kernel<DT, NB, false><<<grid, 256, 0, s>>>(a);
+  } else {
+    if (vec) paged_append_kernel<DT, NB, true><<<grid, 256, 0, s>>>(a);
+    else paged_append_kernel<DT, NB, false><<<grid, 256, 0, s>>>(a);
+  }
+}
+template <int DT>
+void launch_rows_of(const RowArgs& a, bool vec, hipStream_t s) {
+  switch (a.pages.head_dim) {
+    case 32: return launch_rows_as<DT, 1>(a, vec, s);
+    case 64: return launch_rows_as<DT, 2>(a, vec, s);
+    case 96: return launch_rows_as<DT, 3>(a, vec, s);
+    case 128: return launch_rows_as<DT, 4>(a, vec, s);
+    case 192: return launch_rows_as<DT, 6>(a, vec, s);
+    case 256: return launch_rows_as<DT, 8>(a, vec, s);
+  }
+}
+hipError_t launch_rows(const RowArgs& a, bool vec, hipStream_t s) {
+  switch (a.pages.dtype) {
+    case ELMH_F32: launch_rows_of<ELMH_F32>(a, vec, s); break;
+    case ELMH_F16: launch_rows_of<ELMH_F16>(a, vec, s); break;
+    case ELMH_BF16: launch_rows_of<ELMH_BF16>(a, vec, s); break;
+    case ELMH_Q8: launch_rows_of<ELMH_Q8>(a, vec, s); break;
+    case ELMH_Q4: launch_rows_of<ELMH_Q4>(a, vec, s); break;
+  }
+  return hipGetLastError();
+}
+// Rows that can be read or written 16 bytes at a time
+bool rows_aligned(const RowArgs& a, const float* k, const float* v) {
+  return aligned16(k) && aligned16(v) && a.row % 4 == 0 && a.head % 4 == 0;
 }
 
 }  // namespace
@@ -870,11 +1060,23 @@ hipError_t launch_rope_table(float* cs, float* sn, int64_t pos0, int64_t n, int 
 
 hipError_t launch_rope(const float* x, float* y, int T, int n_heads, int hd, int64_t x_row, int64_t y_row,
                        const elmh_rope& rope, const int32_t* pos, int64_t pos0, hipStream_t s) {
-  const int64_t pairs = (int64_t)T * n_heads * (hd / 2), width = (int64_t)n_heads * hd;
-  const int64_t blocks = (pairs + 255) / 256;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  rope_kernel<<<(unsigned)blocks, 256, 0, s>>>(x, y, pairs, n_heads, hd, x_row ? x_row : width, y_row ? y_row : width,
-                                               rope.cos, rope.sin, rope.max_pos, rope.rot_dim, rope.interleaved, pos, pos0);
+  const int64_t width = (int64_t)n_heads * hd;
+  if (!x_row) x_row = width;
+  if (!y_row) y_row = width;
+  const bool inter = rope.interleaved != 0;
+  const bool quads = hd % 4 == 0 && rope.rot_dim % (inter ? 4 : 8) == 0 && x_row % 4 == 0 && y_row % 4 == 0 && aligned16(x) &&
+                     aligned16(y) && aligned16(rope.cos) && aligned16(rope.sin);
+  const int per_head = !quads ? hd / 2 : inter ? hd / 4 : rope.rot_dim / 8 + (hd - rope.rot_dim) / 4;
+  const int64_t blocks = ((int64_t)n_heads * per_head + 255) / 256;
+  // some 8192 workgroups are enough to fill the card
+  const int64_t rows = std::max<int64_t>(1, std::min<int64_t>((T + kRopeRows - 1) / kRopeRows, 8192 / blocks));
+  const dim3 grid((unsigned)blocks, (unsigned)rows);
+  if (quads)
+    rope_quads_kernel<<<grid, 256, 0, s>>>(x, y, T, per_head, n_heads, hd, x_row, y_row, rope.cos, rope.sin, rope.max_pos,
+                                           rope.rot_dim, rope.interleaved, pos, pos0);
+  else
+    rope_pairs_kernel<<<grid, 256, 0, s>>>(x, y, T, per_head, n_heads, hd, x_row, y_row, rope.cos, rope.sin, rope.max_pos,
+                                           rope.rot_dim, rope.interleaved, pos, pos0);
   return hipGetLastError();
 }
 
@@ -884,8 +1086,9 @@ hipError_t launch_paged_append(const float* k, const float* v, int n, int64_t ro
   RowArgs a = row_args(n, row, head, pages, table, n_seqs, max_pages, pos, seq, rope);
   a.k = k;
   a.v = v;
-  paged_append_kernel<<<row_grid(a), 256, 0, s>>>(a);
-  return hipGetLastError();
+  const bool turns = !rope || (aligned16(rope->cos) && aligned16(rope->sin) &&
+                               (rope->interleaved ? rope->rot_dim % 4 == 0 : rope->rot_dim % 8 == 0));
+  return launch_rows(a, turns && rows_aligned(a, k, v), s);
 }
 
 hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t head, const elmh_kv_pages& pages,
@@ -894,8 +1097,7 @@ hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t hea
   RowArgs a = row_args(n, row, head, pages, table, n_seqs, max_pages, pos, seq, nullptr);
   a.ko = k;
   a.vo = v;
-  paged_read_kernel<<<row_grid(a), 256, 0, s>>>(a);
-  return hipGetLastError();
+  return launch_rows(a, rows_aligned(a, k, v), s);
 }
 
 int paged_attention_parts(int n_seqs, int n_heads, int n_kv, int max_len) {
