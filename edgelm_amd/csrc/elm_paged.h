@@ -18,6 +18,7 @@ namespace elmh {
 // ---------------------------------------------------------------- layout
 
 constexpr int kPageStep = 16;   // pages hold a multiple of this many positions: one matrix-instruction tile of tokens
+constexpr int kMaxPositions = 1 << 28;  // of a sequence
 constexpr int kSplitUnit = 32;  // tokens a wave takes at a time; a sequence is split at multiples of it
 
 ELM_HD bool kv_quantized(int dtype) { return dtype == ELMH_Q8 || dtype == ELMH_Q4; }
@@ -40,10 +41,22 @@ ELM_HD int64_t kv_scale(int64_t page, int head, int slot, int n_kv, int page_siz
 ELM_HD int q4_key_byte(int d, int head_dim) { return (d % 32 / 8) * (head_dim / 8) + d / 32 * 4 + d % 8 / 2; }
 ELM_HD int q4_value_byte(int d, int head_dim) { return d % 32 / 2 * (head_dim / 32) + d / 32; }
 
+// 16-position steps over steps a page, without a division: step * page_magic(page_size) / 2^32, exact below 2^24 steps (the
+// magic number is over 2^32 / steps by less than one part, so the product by less than 2^24 * 256 / 2^32 of a page)
+ELM_HD uint32_t page_magic(int page_size) {
+  const uint32_t per = (uint32_t)page_size / kPageStep;
+  return per == 1 ? 0 : (uint32_t)(((uint64_t(1) << 32) + per - 1) / per);
+}
+ELM_HD int page_index(int pos, uint32_t magic) {
+  const uint32_t step = (uint32_t)pos / kPageStep;
+  return magic ? (int)(((uint64_t)step * magic) >> 32) : (int)step;
+}
+
 // The page of position pos in a sequence's row of the table, or -1: no such entry, or no such page
-ELM_HD int64_t kv_page_of(const int32_t* table_row, int max_pages, int64_t n_pages, int pos, int page_size) {
-  const int i = pos / page_size;
-  if (pos < 0 || i >= max_pages) return -1;
+ELM_HD int64_t kv_page_of(const int32_t* table_row, int max_pages, int64_t n_pages, int pos, uint32_t magic) {
+  if (pos < 0 || pos >= kMaxPositions) return -1;
+  const int i = page_index(pos, magic);
+  if (i >= max_pages) return -1;
   const int64_t p = table_row[i];
   return p >= 0 && p < n_pages ? p : -1;
 }
@@ -104,7 +117,7 @@ inline PagedFault check_rope(const elmh_rope* r, int head_dim) {
 inline PagedFault check_table(const int32_t* table, int n_seqs, int max_pages, int page_size) {
   if (!table) return {ELMH_ERR_ARG, "null page table"};
   if (n_seqs < 1 || max_pages < 1) return {ELMH_ERR_ARG, "n_seqs and max_pages are at least 1"};
-  if ((int64_t)max_pages * page_size > INT32_MAX) return {ELMH_ERR_ARG, "max_pages * page_size past 2^31 - 1 positions"};
+  if ((int64_t)max_pages * page_size > kMaxPositions) return {ELMH_ERR_ARG, "max_pages * page_size past 2^28 positions"};
   return {};
 }
 

@@ -5,7 +5,9 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
+#include "elm_dma.h"
 #include "elm_dpp.h"
 #include "elm_paged.h"
 #include "elm_quant.h"
@@ -200,6 +202,7 @@ struct RowArgs {
   const int32_t *pos, *seq;
   const float *cs, *sn;
   int max_pos, rot, inter;
+  uint32_t magic;  // page_magic(page_size)
 };
 
 // Where row i of a call lies in the cache; page < 0: the row is skipped
@@ -210,8 +213,8 @@ struct RowPlace {
 __device__ __forceinline__ RowPlace row_place(const RowArgs& a, int i) {
   const int pos = a.pos[i], seq = a.seq ? a.seq[i] : i;
   if (seq < 0 || seq >= a.n_seqs || pos < 0 || (a.cs && pos >= a.max_pos)) return {-1, 0, 0};
-  const int ps = a.pages.page_size;
-  return {kv_page_of(a.table + (int64_t)seq * a.max_pages, a.max_pages, a.pages.n_pages, pos, ps), pos % ps, pos};
+  return {kv_page_of(a.table + (int64_t)seq * a.max_pages, a.max_pages, a.pages.n_pages, pos, a.magic),
+          pos - page_index(pos, a.magic) * a.pages.page_size, pos};
 }
 
 // Value d of a head's row x, rotated
@@ -432,9 +435,20 @@ __global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a) {
 
 // ---------------------------------------------------------------- attention of one new token a sequence
 
+// f(0), f(1), ..., f(N - 1) with compile-time indices
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, I + 1>(f);
+  }
+}
+
 constexpr int kPaWaves = 4;
 constexpr int kPaHeads = 16;       // query heads a workgroup takes: the columns of a 16 x 16 tile
 constexpr int kPaLeastUnits = 4;   // of a part: one unit a wave
+constexpr int kPaWorkgroups = 1024;  // a call is split into: four a CU
+constexpr int kPaMostParts = 512;    // of a sequence
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // The matrix instructions take 16-bit operands, 32 values deep, or f32 ones, 4 deep. Products are exact in both (f32
@@ -457,13 +471,14 @@ __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
 }
 
 // x[0..7] as the pieces of a 32-deep operand. f16: |x| < 2^15.
+// minus_one: -1, opaque to the compiler, which then takes a residual in one mixed-precision instruction.
 template <int OP>
-__device__ __forceinline__ void split8(const float* x, u32x4* out) {
+__device__ __forceinline__ void split8(const float* x, u32x4* out, float minus_one) {
   if constexpr (OP == kOpF16) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const auto p = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-      const f16x2 r{(_Float16)(x[2 * i] - (float)p[0]), (_Float16)(x[2 * i + 1] - (float)p[1])};
+      const f16x2 r{(_Float16)fmaf((float)p[0], minus_one, x[2 * i]), (_Float16)fmaf((float)p[1], minus_one, x[2 * i + 1])};
       out[0][i] = __builtin_bit_cast(uint32_t, p);
       out[1][i] = __builtin_bit_cast(uint32_t, r);
     }
@@ -486,19 +501,19 @@ __device__ __forceinline__ void split8(const float* x, u32x4* out) {
   }
 }
 
-// int8 levels as f16: the byte u = q + 128 under the exponent of 1024 is 1024 + u, minus 1152 gives q. w: pairs of bytes in the
-// low halves' low bytes.
-__device__ __forceinline__ uint32_t f16_add(uint32_t w, float add) {
-  const f16x2 v = __builtin_bit_cast(f16x2, w) + f16x2{(_Float16)add, (_Float16)add};
-  return __builtin_bit_cast(uint32_t, v);
-}
-// nibbles n at bits 0-3 of each half: 1024 + n - 1032; at bits 4-7: (1024 + 16 n) / 16 - 72
-__device__ __forceinline__ uint32_t f16_low_nibbles(uint32_t w) { return f16_add((w & 0x000F000Fu) | 0x64006400u, -1032.f); }
-__device__ __forceinline__ uint32_t f16_high_nibbles(uint32_t w) {
-  const f16x2 v = __builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u);
-  const f16x2 r = __builtin_elementwise_fma(v, f16x2{(_Float16)0.0625f, (_Float16)0.0625f}, f16x2{(_Float16)-72.f, (_Float16)-72.f});
+// Levels as f16, two an instruction. A small integer u in the low bits of a half is the subnormal u 2^-24, and the fused
+// multiply-add takes it to (u - bias) 2^-9, exactly: levels are held times 2^-9 (kLevelExp), which the final factor undoes.
+constexpr int kLevelExp = 9;
+__device__ __forceinline__ uint32_t f16_levels(uint32_t w, float mul, float add) {
+  const f16x2 r = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)mul, (_Float16)mul},
+                                            f16x2{(_Float16)add, (_Float16)add});
   return __builtin_bit_cast(uint32_t, r);
 }
+// bytes q + 128 in the halves' low bytes
+__device__ __forceinline__ uint32_t f16_bytes(uint32_t w) { return f16_levels(w, 0x1p15f, -0x1p-2f); }
+// nibbles q + 8 at bits 0-3, and at bits 4-7 (16 u 2^-24 times 2^11)
+__device__ __forceinline__ uint32_t f16_low_nibbles(uint32_t w) { return f16_levels(w & 0x000F000Fu, 0x1p15f, -0x1p-6f); }
+__device__ __forceinline__ uint32_t f16_high_nibbles(uint32_t w) { return f16_levels(w & 0x00F000F0u, 0x1p11f, -0x1p-6f); }
 
 // ---- which values of a row a lane holds. Lane = 16 g + n.
 // Keys (rows of the 16 x 32 operand are tokens, n): step j's eight values of lane group g.
@@ -558,29 +573,38 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   }
 }
 
-// row: this lane's token's key row
+// The loads take a uniform base (scalar registers) and a lane's 32-bit offset.
+// base: the block's first key row; off: the lane's row and group, key_offset
 template <int DT, int NB>
-__device__ __forceinline__ void load_key(const uint8_t* row, int g, uint32_t (&w)[key_words(DT, NB)]) {
+__device__ __forceinline__ uint32_t key_offset(int n, int g) {
+  constexpr int HD = 32 * NB;
+  if (DT == ELMH_F32) return n * 4 * HD + 16 * g;
+  if (DT == ELMH_Q8) return n * HD;
+  if (DT == ELMH_Q4) return n * (HD / 2) + 4 * NB * g;
+  return n * 2 * HD + 16 * g;
+}
+template <int DT, int NB>
+__device__ __forceinline__ void load_key(const uint8_t* base, uint32_t off, int g, uint32_t (&w)[key_words(DT, NB)]) {
   if constexpr (DT == ELMH_F32) {
 #pragma unroll
-    for (int j = 0; j < 2 * NB; ++j) load_words<4>(row + 64 * j + 16 * g, w + 4 * j);
+    for (int j = 0; j < 2 * NB; ++j) load_words<4>(base + off + 64 * j, w + 4 * j);
   } else if constexpr (DT == ELMH_Q8) {
 #pragma unroll
-    for (int j = 0; j + 1 < NB; j += 2) load_words<4>(row + 32 * j + 16 * g, w + 2 * j);
-    if constexpr (NB % 2) load_words<2>(row + 32 * (NB - 1) + 8 * g, w + 2 * (NB - 1));
+    for (int j = 0; j + 1 < NB; j += 2) load_words<4>(base + (off + 16 * g) + 32 * j, w + 2 * j);
+    if constexpr (NB % 2) load_words<2>(base + (off + 8 * g) + 32 * (NB - 1), w + 2 * (NB - 1));
   } else if constexpr (DT == ELMH_Q4) {
     if constexpr (NB == 3) {  // 12 g: not on 8 bytes
 #pragma unroll
-      for (int j = 0; j < NB; ++j) w[j] = *reinterpret_cast<const uint32_t*>(row + 12 * g + 4 * j);
+      for (int j = 0; j < NB; ++j) w[j] = *reinterpret_cast<const uint32_t*>(base + off + 4 * j);
     } else if constexpr (NB == 6) {  // 24 g: on 8
 #pragma unroll
-      for (int j = 0; j < NB; j += 2) load_words<2>(row + 24 * g + 4 * j, w + j);
+      for (int j = 0; j < NB; j += 2) load_words<2>(base + off + 4 * j, w + j);
     } else {
-      load_words<NB>(row + 4 * NB * g, w);
+      load_words<NB>(base + off, w);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) load_words<4>(row + 64 * j + 16 * g, w + 4 * j);
+    for (int j = 0; j < NB; ++j) load_words<4>(base + off + 64 * j, w + 4 * j);
   }
 }
 // the operand of step j (16-bit forms)
@@ -591,8 +615,8 @@ __device__ __forceinline__ u32x4 key_operand(const uint32_t (&w)[key_words(DT, N
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t u = w[2 * j + i] ^ 0x80808080u;
-      o[2 * i] = f16_add(__builtin_amdgcn_perm(u, 0x64646464u, 0x00050004), -1152.f);
-      o[2 * i + 1] = f16_add(__builtin_amdgcn_perm(u, 0x64646464u, 0x00070006), -1152.f);
+      o[2 * i] = f16_bytes(__builtin_amdgcn_perm(0, u, 0x0C010C00));
+      o[2 * i + 1] = f16_bytes(__builtin_amdgcn_perm(0, u, 0x0C030C02));
     }
     return o;
   } else if constexpr (DT == ELMH_Q4) {
@@ -603,33 +627,34 @@ __device__ __forceinline__ u32x4 key_operand(const uint32_t (&w)[key_words(DT, N
   }
 }
 
-// row: a token's value row; lane n's part of it
+// row: a token's value row less the lane's offset, off; n: the lane's part of it
 template <int DT, int NB>
-__device__ __forceinline__ void load_value(const uint8_t* row, int n, uint32_t (&w)[value_words(DT, NB)]) {
+__device__ __forceinline__ void load_value(const uint8_t* row, uint32_t off, int n, uint32_t (&w)[value_words(DT, NB)]) {
   if constexpr (DT == ELMH_Q4) {  // NB bytes at n * NB
     if constexpr (NB == 1) {
-      w[0] = row[n];
+      w[0] = row[off + n];
     } else if constexpr (NB == 2) {
-      w[0] = *reinterpret_cast<const uint16_t*>(row + 2 * n);
+      w[0] = *reinterpret_cast<const uint16_t*>(row + (off + 2 * n));
     } else if constexpr (NB == 3) {
-      w[0] = row[3 * n] | row[3 * n + 1] << 8 | row[3 * n + 2] << 16;
+      const uint8_t* p = row + (off + 3 * n);
+      w[0] = p[0] | p[1] << 8 | p[2] << 16;
     } else if constexpr (NB == 6) {
-      const uint16_t* p = reinterpret_cast<const uint16_t*>(row + 6 * n);
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(row + (off + 6 * n));
       w[0] = p[0] | (uint32_t)p[1] << 16;
       w[1] = p[2];
     } else {
-      load_words<NB / 4>(row + NB * n, w);
+      load_words<NB / 4>(row + (off + NB * n), w);
     }
   } else {
     constexpr int B = DT == ELMH_F32 ? 4 : DT == ELMH_Q8 ? 1 : 2;
     // units of 4, 2 and 1 times 32 values
-    if constexpr (NB >= 4) load_words<2 * B>(row + 8 * B * n, w);
-    if constexpr (NB == 8) load_words<2 * B>(row + 128 * B + 8 * B * n, w + 2 * B);
+    if constexpr (NB >= 4) load_words<2 * B>(row + (off + 8 * B * n), w);
+    if constexpr (NB == 8) load_words<2 * B>(row + (off + 8 * B * n) + 128 * B, w + 2 * B);
     constexpr int done = NB / 4 * 4;
-    if constexpr ((NB & 2) != 0) load_words<B>(row + 32 * done * B + 4 * B * n, w + done * B / 2);
+    if constexpr ((NB & 2) != 0) load_words<B>(row + (off + 4 * B * n) + 32 * done * B, w + done * B / 2);
     constexpr int last = NB & ~1;
     if constexpr ((NB & 1) != 0) {
-      const uint8_t* p = row + 32 * last * B + 2 * B * n;
+      const uint8_t* p = row + (off + 2 * B * n) + 32 * last * B;
       if constexpr (B == 1) w[last / 2] = *reinterpret_cast<const uint16_t*>(p);
       else load_words<B / 2>(p, w + last * B / 2);
     }
@@ -644,7 +669,7 @@ __device__ __forceinline__ u32x4 value_operand(const uint32_t (&v)[8][value_word
     if constexpr (DT == ELMH_Q8) {
       const uint32_t a = v[2 * i][x / 4], b = v[2 * i + 1][x / 4];
       const uint32_t sel = 0x0C040C00u + (x % 4) * 0x00010001u;
-      o[i] = f16_add(__builtin_amdgcn_perm(b, a, sel) | 0x64006400u, -1152.f);  // the bytes were loaded and flipped
+      o[i] = f16_bytes(__builtin_amdgcn_perm(b, a, sel));  // the bytes were flipped to q + 128
     } else if constexpr (DT == ELMH_Q4) {
       const int j = x / 2;
       const uint32_t sel = 0x0C040C00u + (j % 4) * 0x00010001u;
@@ -665,6 +690,7 @@ struct PagedAttnArgs {
   elmh_kv_pages pages;
   const int32_t* table;
   int max_pages;
+  uint32_t magic;  // page_magic(page_size)
   const int32_t* lens;
   int max_len;
   const float *cs, *sn;
@@ -674,16 +700,36 @@ struct PagedAttnArgs {
   float* part_s;  // [seq][head][part][2]: running maximum (base 2), sum
 };
 
+// max over the four lane groups: v_permlane16_swap of a value with itself leaves each lane its own and its neighbour row's
 __device__ __forceinline__ float max_over_groups(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+
+// Two blocks of 16 tokens (a wave's step): where they lie, and how many tokens of each count (0: behind the end, or no page)
+struct PagedTile {
+  int valid[2];
+  int64_t row[2], scale[2];
+};
+
+// What a wave holds of a tile while it is on its way
+template <int DT, int NB>
+struct PagedRegs {
+  uint32_t k[2][key_words(DT, NB)];
+  uint32_t v[8][value_words(DT, NB)];
+  f32x4 ks, vs;  // quantized: lane n of a group has the scales of group n / 2 of block n % 2 (n < 2 NB; q8: of block n % 2)
+};
 
 // One workgroup: one part of one sequence's cache for up to 16 query heads of one kv head, its waves taking 32 tokens at a time.
 // Scores as K Q^T (tokens x heads) leave a lane with four tokens of one head, which is what the second product V^T P^T takes
 // as its operand: no exchange between lanes but the maximum over the four lane groups. One pass: running maximum m and sum l.
+// A wave's next keys are on their way while it takes the weights and the values, its next values while it takes the scores.
+// Bound by reading the cache where it is long, by the way to the first rows where it is short.
 template <int DT, int NB>
-__global__ __launch_bounds__(64 * kPaWaves) void paged_attention_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int HD = 32 * NB, OP = op_of(DT), PC = pieces_of(DT);
   extern __shared__ float lds[];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
@@ -692,13 +738,73 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attention_kernel(PagedAtt
   const int h0 = kvh * a.group + blockIdx.y % a.head_tiles * kPaHeads;
   const int heads = min(kPaHeads, (kvh + 1) * a.group - h0);
   const elmh_kv_pages& pg = a.pages;
-  const int len = min(max(a.lens[seq], 0), a.max_len);
+  const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[seq], 0), a.max_len));
   const int units = (len + kSplitUnit - 1) / kSplitUnit;
   const int per = split_size(units, a.parts, kPaLeastUnits), live = split_parts(units, per);
   float* out = a.out + (int64_t)seq * a.n_heads * HD + (int64_t)h0 * HD;
-  if (len == 0 && part == 0)
-    for (int i = tid; i < heads * HD; i += 64 * kPaWaves) out[i] = 0.f;
-  if (part >= live) return;
+  if (part >= live) {
+    if (part == 0)  // an empty sequence
+      for (int i = tid; i < heads * HD; i += 64 * kPaWaves) out[i] = 0.f;
+    return;
+  }
+
+  const int32_t* trow = a.table + (int64_t)seq * a.max_pages;
+  const int ps = pg.page_size, last = (len - 1) / kPageStep;
+  constexpr int RB = DT == ELMH_F32 ? 4 * HD : DT == ELMH_Q8 ? HD : DT == ELMH_Q4 ? HD / 2 : 2 * HD;
+  constexpr int NG = DT == ELMH_Q8 ? 1 : DT == ELMH_Q4 ? NB : 0;
+  const uint8_t* kpool = static_cast<const uint8_t*>(pg.k);
+  const uint8_t* vpool = static_cast<const uint8_t*>(pg.v);
+  const uint32_t koff = key_offset<DT, NB>(n, g), voff = 4 * g * RB;
+  // the lane's scales: group j of block u, as PagedRegs says
+  const int sj = NG > 1 ? min(n / 2, NG - 1) : 0, su = n & 1;
+  const uint32_t soff = (uint32_t)(sj * ps + 4 * g) * 4;
+
+  // the table's entries of a unit's two blocks (of the last block's, past the end)
+  const auto ask = [&](int unit, int (&id)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) id[u] = trow[page_index(min(2 * unit + u, last) * kPageStep, a.magic)];
+  };
+  const auto place = [&](int unit, const int (&id)[2]) {
+    PagedTile t;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int block = min(2 * unit + u, last), pos = block * kPageStep;
+      const int page = __builtin_amdgcn_readfirstlane(id[u]);
+      const bool there = (uint32_t)page < (uint32_t)pg.n_pages;
+      t.valid[u] = there && 2 * unit + u <= last ? min(kPageStep, len - pos) : 0;
+      const int64_t head = (int64_t)(there ? page : 0) * pg.n_kv + kvh;
+      const int slot = pos - page_index(pos, a.magic) * ps;
+      t.row[u] = head * ps + slot;
+      t.scale[u] = head * NG * ps + slot;
+    }
+    return t;
+  };
+  PagedRegs<DT, NB> r;
+  const auto load_keys = [&](const PagedTile& t) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_key<DT, NB>(kpool + t.row[u] * RB, koff, g, r.k[u]);
+    if constexpr (NG > 0) r.ks = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(pg.k_scale + (su ? t.scale[1] : t.scale[0])) + soff);
+  };
+  const auto load_values = [&](const PagedTile& t) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load_value<DT, NB>(vpool + t.row[u] * RB + i * RB, voff, n, r.v[4 * u + i]);
+    if constexpr (NG > 0) r.vs = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(pg.v_scale + (su ? t.scale[1] : t.scale[0])) + soff);
+  };
+
+  const int end = min(units, (part + 1) * per);
+  int unit = part * per + wave;
+  const bool busy = unit < end;  // a wave without a unit joins with nothing
+  int id[2];
+  PagedTile tile;
+  if (busy) {
+    ask(unit, id);
+    tile = place(unit, id);
+    load_keys(tile);
+    load_values(tile);
+    ask(unit + kPaWaves, id);
+  }
 
   // the queries, rotated at the last position
   const float* q = a.q + seq * a.q_row + (int64_t)h0 * HD;
@@ -706,8 +812,10 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attention_kernel(PagedAtt
     const int64_t at = (int64_t)(len - 1) * (a.rot / 2);
     lds[i] = a.cs ? rotated(q + i / HD * HD, i % HD, a.cs + at, a.sn + at, a.rot / 2, a.inter) : q[i];
   }
-  __syncthreads();
+  lds_barrier();
   // as operands; `scale`: what a product is multiplied by to be a score in units of log2
+  float minus_one = -1.f;
+  asm("" : "+v"(minus_one));
   float scale = kLog2e / sqrtf((float)HD);
   u32x4 qo[OP == kOpF32 ? 1 : NB][OP == kOpF32 ? 1 : PC];
   float qf[OP == kOpF32 ? 8 * NB : 1];
@@ -726,130 +834,90 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attention_kernel(PagedAtt
 #pragma unroll
         for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qrow[32 * j + 8 * g + e]));
       big = max_over_groups(big);
-      const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -110), 110);
-      up = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
-      scale *= __uint_as_float((uint32_t)(127 - 9 + ex) << 23);
+      const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 100);
+      up = pow2(9 - ex);
+      scale *= pow2(ex - 9 + (NG ? kLevelExp : 0));
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = qrow[key_dim<DT, NB>(j, g, e)] * up;
-      split8<OP>(x, qo[j]);
+      split8<OP>(x, qo[j], minus_one);
     }
   }
 
-  const int32_t* trow = a.table + (int64_t)seq * a.max_pages;
-  const int ps = pg.page_size;
-  constexpr int RB = DT == ELMH_F32 ? 4 * HD : DT == ELMH_Q8 ? HD : DT == ELMH_Q4 ? HD / 2 : 2 * HD;
-  constexpr int NG = DT == ELMH_Q8 ? 1 : DT == ELMH_Q4 ? NB : 0;
-  const uint8_t* kpool = static_cast<const uint8_t*>(pg.k);
-  const uint8_t* vpool = static_cast<const uint8_t*>(pg.v);
   float m = -INFINITY, l = 0.f;
-  int vexp = -112;  // q8, q4: the softmax weights take the value scales over 2^vexp, the largest seen
+  int vexp = -100;  // q8, q4: the softmax weights take the value scales over 2^vexp, the largest seen
   f32x4 acc[2 * NB];
 #pragma unroll
   for (int x = 0; x < 2 * NB; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const int end = min(units, (part + 1) * per);
-  for (int unit = part * per + wave; unit < end; unit += kPaWaves) {
-    int valid[2];
-    int64_t row[2], srow[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int pos = unit * kSplitUnit + 16 * u;
-      const int64_t page = pos < len ? kv_page_of(trow, a.max_pages, pg.n_pages, pos, ps) : -1;
-      valid[u] = page >= 0 ? min(16, len - pos) : 0;
-      row[u] = kv_row(page >= 0 ? page : 0, kvh, page >= 0 ? pos % ps : 0, pg.n_kv, ps);
-      srow[u] = kv_scale(page >= 0 ? page : 0, kvh, page >= 0 ? pos % ps : 0, pg.n_kv, ps, NG);
-    }
-    const bool whole = valid[0] == 16 && valid[1] == 16;
-
+  const auto step = [&](auto more) {
+    const bool whole = tile.valid[0] == kPageStep && tile.valid[1] == kPageStep;
     float s[8];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      uint32_t w[key_words(DT, NB)];
-      load_key<DT, NB>(kpool + (row[u] + n) * RB, g, w);
+    static_for<2>([&](auto U) {
+      constexpr int u = U;
       f32x4 sc{0.f, 0.f, 0.f, 0.f};
       if constexpr (OP == kOpF32) {
 #pragma unroll
-        for (int j = 0; j < 8 * NB; ++j) sc = mfma_f32(__uint_as_float(w[j]), qf[j], sc);
+        for (int j = 0; j < 8 * NB; ++j) sc = mfma_f32(__uint_as_float(r.k[u][j]), qf[j], sc);
       } else {
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          const u32x4 ko = key_operand<DT, NB>(w, j);
+        static_for<NB>([&](auto J) {
+          constexpr int j = J;
+          const u32x4 ko = key_operand<DT, NB>(r.k[u], j);
           f32x4 t = DT == ELMH_Q4 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc;
 #pragma unroll
           for (int p = PC - 1; p >= 0; --p) t = mfma<OP>(ko, qo[j][p], t);
           if constexpr (DT == ELMH_Q4) {
-            const f32x4 ks = *reinterpret_cast<const f32x4*>(pg.k_scale + srow[u] + (int64_t)j * ps + 4 * g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sc[r] = fmaf(t[r], ks[r], sc[r]);
+            for (int i = 0; i < 4; ++i) sc[i] = fmaf(row_bcast<2 * j + u>(r.ks[i]), t[i], sc[i]);
           } else {
             sc = t;
           }
-        }
-      }
-      if constexpr (DT == ELMH_Q8) {
-        const f32x4 ks = *reinterpret_cast<const f32x4*>(pg.k_scale + srow[u] + 4 * g);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sc[r] *= ks[r];
+        });
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[4 * u + r] = 4 * g + r < valid[u] ? sc[r] * scale : -INFINITY;
+      for (int i = 0; i < 4; ++i) s[4 * u + i] = DT == ELMH_Q8 ? sc[i] * (row_bcast<u>(r.ks[i]) * scale) : sc[i] * scale;
+    });
+    const PagedTile now = tile;
+    if constexpr (more) {
+      unit += kPaWaves;
+      tile = place(unit, id);
+      load_keys(tile);
+      ask(unit + kPaWaves, id);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = 4 * g + i % 4 < now.valid[i / 4] ? s[i] : -INFINITY;
     }
 
-    float top = s[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
+    const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
     const float mn = fmaxf(m, max_over_groups(top));
     const float ref = mn == -INFINITY ? 0.f : mn;  // no token so far: weights of 0, not of exp(-inf + inf)
     float p[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
-    }
+    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
     float fade = __builtin_amdgcn_exp2f(m - ref);
     m = mn;
-    l = l * fade + ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    l = l * fade + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
 
-    uint32_t v[8][value_words(DT, NB)];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) load_value<DT, NB>(vpool + (row[u] + 4 * g + r) * RB, n, v[4 * u + r]);
-    if constexpr (DT == ELMH_Q8) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int k = 0; k < value_words(DT, NB); ++k) v[i][k] ^= 0x80808080u;
-    }
-    if constexpr (NG == 0) {  // a slot behind the end may hold a NaN, which a weight of 0 does not remove
-      if (!whole) {
+    if (!whole) {
+      if constexpr (NG == 0) {  // a slot behind the end may hold a NaN, which a weight of 0 does not remove
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int k = 0; k < value_words(DT, NB); ++k) v[i][k] = 4 * g + i % 4 < valid[i / 4] ? v[i][k] : 0u;
+          for (int k = 0; k < value_words(DT, NB); ++k) r.v[i][k] = 4 * g + i % 4 < now.valid[i / 4] ? r.v[i][k] : 0u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.vs[i] = 4 * g + i < (su ? now.valid[1] : now.valid[0]) ? r.vs[i] : 0.f;
       }
     }
-    float vs[NG ? NG : 1][8];
     if constexpr (NG > 0) {
-      float big = 0.f;
-#pragma unroll
-      for (int j = 0; j < NG; ++j)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const f32x4 t = *reinterpret_cast<const f32x4*>(pg.v_scale + srow[u] + (int64_t)j * ps + 4 * g);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            vs[j][4 * u + r] = 4 * g + r < valid[u] ? t[r] : 0.f;
-            big = fmaxf(big, fabsf(vs[j][4 * u + r]));
-          }
-        }
-      if (__any(big > __uint_as_float((uint32_t)(127 + vexp) << 23))) {  // rare after the first tokens
-        const int ex = min((int)(__float_as_uint(wave_max(big)) >> 23) - 126, 120);
-        const int by = min(ex - vexp, 126);
-        fade *= __uint_as_float((uint32_t)(127 - by) << 23);
+      const float big = fmaxf(fmaxf(fabsf(r.vs[0]), fabsf(r.vs[1])), fmaxf(fabsf(r.vs[2]), fabsf(r.vs[3])));
+      if (__any(big > pow2(vexp))) {  // rare after the first tokens
+        const int ex = min((int)(__float_as_uint(wave_max(big)) >> 23) - 126, 100);
+        fade *= pow2(max(vexp - ex, -126));
         vexp = ex;
       }
     }
@@ -857,56 +925,76 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attention_kernel(PagedAtt
 #pragma unroll
       for (int x = 0; x < 2 * NB; ++x)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[x][r] *= fade;
+        for (int i = 0; i < 4; ++i) acc[x][i] *= fade;
     }
 
     if constexpr (OP == kOpF32) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int x = 0; x < 2 * NB; ++x) acc[x] = mfma_f32(__uint_as_float(v[i][x]), p[i], acc[x]);
+        for (int x = 0; x < 2 * NB; ++x) acc[x] = mfma_f32(__uint_as_float(r.v[i][x]), p[i], acc[x]);
     } else {
       // f16 pieces: weights up to 2^14, so that a weight 2^-28 of the largest is still a normal number
-      const float up = OP == kOpF16 ? (NG ? __uint_as_float((uint32_t)(127 + 14 - vexp) << 23) : 16384.f) : 1.f;
-      u32x4 po[PC];
+      if constexpr (OP == kOpF16) {
+        const float up = pow2(14 - (NG ? vexp : 0));
 #pragma unroll
-      for (int x = 0; x < 2 * NB; ++x) {
-        if (x == 0 || (DT == ELMH_Q4 && x % 2 == 0)) {
-          float t[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) t[i] = NG ? p[i] * (vs[NG > 1 ? x / 2 : 0][i] * up) : p[i] * up;
-          split8<OP>(t, po);
-        }
-        const u32x4 vo = value_operand<DT, NB>(v, x);
-#pragma unroll
-        for (int k = PC - 1; k >= 0; --k) acc[x] = mfma<OP>(vo, po[k], acc[x]);
+        for (int i = 0; i < 8; ++i) p[i] *= up;
       }
+      if constexpr (DT == ELMH_Q8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int k = 0; k < value_words(DT, NB); ++k) r.v[i][k] ^= 0x80808080u;
+      }
+      constexpr int runs = DT == ELMH_Q4 ? NB : 1;  // of values that share their scale
+      static_for<runs>([&](auto J) {
+        constexpr int j = J;
+        u32x4 po[PC];
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          t[i] = NG ? row_bcast<2 * j>(r.vs[i]) * p[i] : p[i];
+          t[4 + i] = NG ? row_bcast<2 * j + 1>(r.vs[i]) * p[4 + i] : p[4 + i];
+        }
+        split8<OP>(t, po, minus_one);
+#pragma unroll
+        for (int x = j * 2 * NB / runs; x < (j + 1) * 2 * NB / runs; ++x) {
+          const u32x4 vo = value_operand<DT, NB>(r.v, x);
+#pragma unroll
+          for (int k = PC - 1; k >= 0; --k) acc[x] = mfma<OP>(vo, po[k], acc[x]);
+        }
+      });
     }
+    if constexpr (more) load_values(tile);
+  };
+  if (busy) {
+    while (unit + kPaWaves < end) step(std::true_type{});
+    step(std::false_type{});
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
   // the waves' sums joined: o = sum_w 2^(m_w - M) o_w
   if constexpr (OP == kOpF16) {
-    const float f = __uint_as_float((uint32_t)(127 + (NG ? vexp : 0) - 14) << 23);
+    const float f = pow2((NG ? vexp + kLevelExp : 0) - 14);
 #pragma unroll
     for (int x = 0; x < 2 * NB; ++x)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[x][r] *= f;
+      for (int i = 0; i < 4; ++i) acc[x][i] *= f;
   }
-  __syncthreads();  // the queries have been read
+  lds_barrier();  // the queries have been read
   float* stat = lds + kPaWaves * heads * HD;
   if (n < heads) {
 #pragma unroll
     for (int x = 0; x < 2 * NB; ++x)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) lds[(wave * heads + n) * HD + value_dim<DT, NB>(x, 4 * g + r)] = acc[x][r];
+      for (int i = 0; i < 4; ++i) lds[(wave * heads + n) * HD + value_dim<DT, NB>(x, 4 * g + i)] = acc[x][i];
     if (g == 0) {
       stat[wave * kPaHeads + n] = m;
       stat[(kPaWaves + wave) * kPaHeads + n] = l;
     }
   }
-  __syncthreads();
+  lds_barrier();
   for (int i = tid; i < heads * HD; i += 64 * kPaWaves) {
     const int h = i / HD, d = i % HD;
     float M = -INFINITY;
@@ -933,24 +1021,58 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_attention_kernel(PagedAtt
   }
 }
 
-// The parts of a (sequence, head) joined, in their order
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
-  const int hd = a.pages.head_dim, d = threadIdx.x, head = blockIdx.x, seq = blockIdx.y;
+// The parts of a (sequence, head) joined, always in the same order: the parts' weights first, then their rows, four values a
+// thread, the threads' sums of every (256 / (head_dim / 4))-th part added in turn.
+constexpr int kJoinThreads = 256;
+template <int NB>
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs a) {
+  constexpr int HD = 32 * NB, Q = HD / 4, G = kJoinThreads / Q;
+  __shared__ float w[kPaMostParts], wave_m[kJoinThreads / 64], wave_l[kJoinThreads / 64];
+  __shared__ f32x4 sum[G][Q];
+  const int tid = threadIdx.x, head = blockIdx.x, seq = blockIdx.y;
   const int len = min(max(a.lens[seq], 0), a.max_len);
   const int units = (len + kSplitUnit - 1) / kSplitUnit;
   const int live = split_parts(units, split_size(units, a.parts, kPaLeastUnits));
-  if (live < 2 || d >= hd) return;
+  if (live < 2) return;
   const int64_t at = ((int64_t)seq * a.n_heads + head) * a.parts;
+  const float* stats = a.part_s + at * 2;
   float M = -INFINITY;
-  for (int s = 0; s < live; ++s) M = fmaxf(M, a.part_s[(at + s) * 2]);
+  for (int s = tid; s < live; s += kJoinThreads) M = fmaxf(M, stats[2 * s]);
+  M = wave_max(M);
+  if ((tid & 63) == 0) wave_m[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
   const float ref = M == -INFINITY ? 0.f : M;
-  float o = 0.f, L = 0.f;
-  for (int s = 0; s < live; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.part_s[(at + s) * 2] - ref);
-    o += f * a.part_o[(at + s) * hd + d];
-    L += f * a.part_s[(at + s) * 2 + 1];
+  float L = 0.f;
+  for (int s = tid; s < live; s += kJoinThreads) {
+    const float f = __builtin_amdgcn_exp2f(stats[2 * s] - ref);
+    w[s] = f;
+    L += f * stats[2 * s + 1];
   }
-  a.out[((int64_t)seq * a.n_heads + head) * hd + d] = L == 0.f ? 0.f : o / L;
+#pragma unroll
+  for (int off = 32; off; off >>= 1) L += __shfl_xor(L, off, 64);
+  if ((tid & 63) == 0) wave_l[tid >> 6] = L;
+  __syncthreads();
+  L = (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]);
+  const int c = tid % Q, grp = tid / Q;
+  if (grp < G) {
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    const f32x4* rows = reinterpret_cast<const f32x4*>(a.part_o + at * HD) + c;
+#pragma unroll 4
+    for (int s = grp; s < live; s += G) {
+      const f32x4 v = rows[(int64_t)s * Q];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += w[s] * v[i];
+    }
+    sum[grp][c] = o;
+  }
+  __syncthreads();
+  if (tid < HD) {
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) o += sum[i][tid / 4][tid % 4];
+    a.out[((int64_t)seq * a.n_heads + head) * HD + tid] = L == 0.f ? 0.f : o / L;
+  }
 }
 
 template <int DT, int NB>
@@ -965,7 +1087,7 @@ hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, hipStre
   paged_attention_kernel<DT, NB><<<grid, 64 * kPaWaves, lds, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
-  paged_join_kernel<<<dim3(a.n_heads, n_seqs), (32 * NB + 63) / 64 * 64, 0, s>>>(a);
+  paged_join_kernel<NB><<<dim3(a.n_heads, n_seqs), kJoinThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 template <int DT>
@@ -994,6 +1116,7 @@ RowArgs row_args(int n, int64_t row, int64_t head, const elmh_kv_pages& pages, c
   a.max_pages = max_pages;
   a.pos = pos;
   a.seq = seq;
+  a.magic = page_magic(pages.page_size);
   if (rope) {
     a.cs = rope->cos;
     a.sn = rope->sin;
@@ -1104,8 +1227,8 @@ int paged_attention_parts(int n_seqs, int n_heads, int n_kv, int max_len) {
   const int tiles = (n_heads / n_kv + kPaHeads - 1) / kPaHeads;
   const int64_t rows = (int64_t)n_seqs * n_kv * tiles;
   const int units = (max_len + kSplitUnit - 1) / kSplitUnit, most = (units + kPaLeastUnits - 1) / kPaLeastUnits;
-  const int64_t want = (2048 + rows - 1) / rows;
-  return (int)(want < most ? want : most);
+  const int64_t want = std::max<int64_t>(1, kPaWorkgroups / rows);
+  return (int)std::min<int64_t>({want, most, kPaMostParts});
 }
 
 size_t paged_attention_scratch_bytes(int n_seqs, int n_heads, int head_dim, int parts) {
@@ -1133,6 +1256,7 @@ hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int
     a.rot = rope->rot_dim;
     a.inter = rope->interleaved;
   }
+  a.magic = page_magic(pages.page_size);
   a.parts = parts;
   a.part_o = scratch;
   a.part_s = scratch + (int64_t)n_seqs * n_heads * parts * pages.head_dim;

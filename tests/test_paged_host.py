@@ -33,7 +33,8 @@ int rope(const float* x, const float* y, int64_t T, int nh, int hd, int64_t xr, 
 int table(const float* c, const float* s, int64_t p0, int64_t n, int rot, double th, const elmh_rope_scaling* sc) {
   return code(check_rope_table(c, s, p0, n, rot, th, sc));
 }
-int64_t page_of(const int32_t* row, int mp, int64_t np, int pos, int ps) { return kv_page_of(row, mp, np, pos, ps); }
+int64_t page_of(const int32_t* row, int mp, int64_t np, int pos, int ps) { return kv_page_of(row, mp, np, pos, page_magic(ps)); }
+int page_index_of(int pos, int ps) { return page_index(pos, page_magic(ps)); }
 int per(int units, int parts, int least) { return split_size(units, parts, least); }
 int parts_of(int units, int per) { return split_parts(units, per); }
 int kbyte(int d, int hd) { return q4_key_byte(d, hd); }
@@ -171,6 +172,16 @@ def test_page_of_a_position(host):
         assert host.page_of(p, len(row), 100, len(row) * ps, ps) == -1
         assert host.page_of(p, len(row), 100, -1, ps) == -1
         assert host.page_of(p, len(row), 100, -2**31, ps) == -1
+        assert host.page_of(p, len(row), 100, 2**31 - 1, ps) == -1
+        assert host.page_of(p, len(row), 100, 2**28, ps) == -1
+
+
+def test_page_index_is_the_quotient(host):
+    """At every page size, positions about each multiple and at the largest."""
+    for ps in range(16, 4097, 16):
+        last = 2**28 - 1
+        for pos in [0, 1, ps - 1, ps, ps + 1, 7 * ps - 1, 7 * ps, last, last - 1, last // ps * ps, last // ps * ps - 1, 2**27 // ps * ps, 2**27 // ps * ps - 1]:
+            assert host.page_index_of(pos, ps) == pos // ps, (pos, ps)
 
 
 def test_parts_cover_a_sequence(host):
