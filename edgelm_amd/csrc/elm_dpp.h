@@ -7,9 +7,9 @@ namespace elmh {
 
 // quad_perm [1,0,3,2] (swap neighbours), quad_perm [2,3,0,1] (swap pairs), row_half_mirror
 // (lane i <- 7 - i within each 8 lanes), row_mirror (lane i <- 15 - i within each 16 lanes),
-// row_ror:8 (lane i <- (i + 8) mod 16 within each 16 lanes)
+// row_ror:8 (lane i <- (i + 8) mod 16 within each 16 lanes), and row_ror:4, row_ror:2
 constexpr int kDppQuadXor1 = 0xB1, kDppQuadXor2 = 0x4E, kDppHalfMirror = 0x141, kDppRowMirror = 0x140,
-              kDppRowRor8 = 0x128;
+              kDppRowRor8 = 0x128, kDppRowRor4 = 0x124, kDppRowRor2 = 0x122;
 
 template <int CTRL>
 __device__ __forceinline__ int dpp_i(int v) {

@@ -96,6 +96,8 @@ inline PagedFault check_kv_pages(const elmh_kv_pages* p) {
   const PagedFault f = check_kv_shape(p->dtype, p->n_kv, p->head_dim, p->page_size);
   if (f.code) return f;
   if (p->n_pages < 1 || p->n_pages > INT32_MAX) return {ELMH_ERR_ARG, "n_pages outside 1 .. 2^31 - 1"};
+  if (p->n_pages * p->n_kv > (int64_t(1) << 32) / (p->page_size / kPageStep) - 1)
+    return {ELMH_ERR_ARG, "a pool of 2^36 rows or more"};
   if (!p->k || !p->v) return {ELMH_ERR_ARG, "null key or value pool"};
   if (!aligned16(p->k) || !aligned16(p->v)) return {ELMH_ERR_ARG, "pools start on 16 bytes"};
   if (kv_quantized(p->dtype)) {

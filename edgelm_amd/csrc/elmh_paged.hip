@@ -447,7 +447,7 @@ __device__ __forceinline__ void static_for(F&& f) {
 constexpr int kPaWaves = 4;
 constexpr int kPaHeads = 16;       // query heads a workgroup takes: the columns of a 16 x 16 tile
 constexpr int kPaLeastUnits = 4;   // of a part: one unit a wave
-constexpr int kPaWorkgroups = 1024;  // a call is split into: four a CU
+constexpr int kPaWorkgroups = 512;   // a call is split into
 constexpr int kPaMostParts = 512;    // of a sequence
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -700,12 +700,14 @@ struct PagedAttnArgs {
   float* part_s;  // [seq][head][part][2]: running maximum (base 2), sum
 };
 
+// One instruction for two or three operands (a NaN stays one), where fmaxf first quiets what may be signalling
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // max over the four lane groups: v_permlane16_swap of a value with itself leaves each lane its own and its neighbour row's
 __device__ __forceinline__ float max_over_groups(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  v = max_of(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return max_of(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
 
@@ -716,11 +718,13 @@ struct PagedTile {
 };
 
 // What a wave holds of a tile while it is on its way
-template <int DT, int NB>
+template <int DT, int NB, bool COLS>
 struct PagedRegs {
   uint32_t k[2][key_words(DT, NB)];
   uint32_t v[8][value_words(DT, NB)];
-  f32x4 ks, vs;  // quantized: lane n of a group has the scales of group n / 2 of block n % 2 (n < 2 NB; q8: of block n % 2)
+  // quantized: of tokens 4 g .. + 3 of a block. COLS: of the lane's group, for both blocks; else lane n has group n / 2 of block
+  // n % 2 (q8: of block n % 2) in [0]
+  f32x4 ks[COLS ? 2 : 1], vs[COLS ? 2 : 1];
 };
 
 // One workgroup: one part of one sequence's cache for up to 16 query heads of one kv head, its waves taking 32 tokens at a time.
@@ -728,7 +732,11 @@ struct PagedRegs {
 // as its operand: no exchange between lanes but the maximum over the four lane groups. One pass: running maximum m and sum l.
 // A wave's next keys are on their way while it takes the weights and the values, its next values while it takes the scores.
 // Bound by reading the cache where it is long, by the way to the first rows where it is short.
-template <int DT, int NB>
+// COLS (q4, where the heads times the NB groups of 32 fit in the 16 columns): column n = h + j 16 / NB is head h and group j. Its
+// query is zero outside the group, so a score's NB parts come out in NB lanes, each multiplied by its own group's scale and
+// then added over them; and its weights take its own group's value scales, so that one split of 8 weights serves in place of
+// NB (344 vector instructions a tile for 476).
+template <int DT, int NB, bool COLS>
 __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int HD = 32 * NB, OP = op_of(DT), PC = pieces_of(DT);
   extern __shared__ float lds[];
@@ -756,41 +764,53 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   const uint8_t* vpool = static_cast<const uint8_t*>(pg.v);
   const uint32_t koff = key_offset<DT, NB>(n, g), voff = 4 * g * RB;
   // the lane's scales: group j of block u, as PagedRegs says
-  const int sj = NG > 1 ? min(n / 2, NG - 1) : 0, su = n & 1;
+  constexpr int HS = COLS ? 16 / NB : 16;
+  const int sj = COLS ? n / HS : NG > 1 ? min(n / 2, NG - 1) : 0, su = n & 1;
   const uint32_t soff = (uint32_t)(sj * ps + 4 * g) * 4;
+  const int qn = COLS ? n % HS : n;  // the lane's head
 
   // the table's entries of a unit's two blocks (of the last block's, past the end)
   const auto ask = [&](int unit, int (&id)[2]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) id[u] = trow[page_index(min(2 * unit + u, last) * kPageStep, a.magic)];
   };
+  const int steps = ps / kPageStep;
   const auto place = [&](int unit, const int (&id)[2]) {
     PagedTile t;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int block = min(2 * unit + u, last), pos = block * kPageStep;
+      const int block = min(2 * unit + u, last);
       const int page = __builtin_amdgcn_readfirstlane(id[u]);
       const bool there = (uint32_t)page < (uint32_t)pg.n_pages;
-      t.valid[u] = there && 2 * unit + u <= last ? min(kPageStep, len - pos) : 0;
-      const int64_t head = (int64_t)(there ? page : 0) * pg.n_kv + kvh;
-      const int slot = pos - page_index(pos, a.magic) * ps;
-      t.row[u] = head * ps + slot;
-      t.scale[u] = head * NG * ps + slot;
+      t.valid[u] = there && 2 * unit + u <= last ? min(kPageStep, len - block * kPageStep) : 0;
+      const uint32_t head = (uint32_t)(there ? page : 0) * pg.n_kv + kvh;
+      const uint32_t step = block - page_index(block * kPageStep, a.magic) * steps;
+      t.row[u] = (int64_t)(head * steps + step) * kPageStep;  // the pool has fewer than 2^32 blocks
+      t.scale[u] = NG == 1 ? t.row[u] : ((int64_t)(head * steps) * NG + step) * kPageStep;
     }
     return t;
   };
-  PagedRegs<DT, NB> r;
+  PagedRegs<DT, NB, COLS> r;
+  const auto load_scales = [&](f32x4* to, const float* pool, const PagedTile& t) {
+    const auto at = [&](int64_t scale) { return *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(pool + scale) + soff); };
+    if constexpr (COLS) {
+      to[0] = at(t.scale[0]);
+      to[1] = at(t.scale[1]);
+    } else if constexpr (NG > 0) {
+      to[0] = at(su ? t.scale[1] : t.scale[0]);
+    }
+  };
   const auto load_keys = [&](const PagedTile& t) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) load_key<DT, NB>(kpool + t.row[u] * RB, koff, g, r.k[u]);
-    if constexpr (NG > 0) r.ks = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(pg.k_scale + (su ? t.scale[1] : t.scale[0])) + soff);
+    load_scales(r.ks, pg.k_scale, t);
   };
   const auto load_values = [&](const PagedTile& t) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) load_value<DT, NB>(vpool + t.row[u] * RB + i * RB, voff, n, r.v[4 * u + i]);
-    if constexpr (NG > 0) r.vs = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(pg.v_scale + (su ? t.scale[1] : t.scale[0])) + soff);
+    load_scales(r.vs, pg.v_scale, t);
   };
 
   const int end = min(units, (part + 1) * per);
@@ -819,7 +839,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   float scale = kLog2e / sqrtf((float)HD);
   u32x4 qo[OP == kOpF32 ? 1 : NB][OP == kOpF32 ? 1 : PC];
   float qf[OP == kOpF32 ? 8 * NB : 1];
-  const float* qrow = lds + min(n, heads - 1) * HD;
+  const float* qrow = lds + min(qn, heads - 1) * HD;
   if constexpr (OP == kOpF32) {
 #pragma unroll
     for (int j = 0; j < 2 * NB; ++j)
@@ -833,17 +853,29 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qrow[32 * j + 8 * g + e]));
-      big = max_over_groups(big);
+      big = max_over_groups(big);  // (with COLS every lane of a head reads all of its groups)
       const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 100);
       up = pow2(9 - ex);
       scale *= pow2(ex - 9 + (NG ? kLevelExp : 0));
     }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
+    if constexpr (COLS) {
       float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = qrow[key_dim<DT, NB>(j, g, e)] * up;
-      split8<OP>(x, qo[j], minus_one);
+      for (int e = 0; e < 8; ++e) x[e] = qrow[32 * sj + key_dim<DT, NB>(0, g, e)] * up;
+      u32x4 o[PC];
+      split8<OP>(x, o, minus_one);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int p = 0; p < PC; ++p) qo[j][p] = sj == j ? o[p] : u32x4{0, 0, 0, 0};
+    } else {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = qrow[key_dim<DT, NB>(j, g, e)] * up;
+        split8<OP>(x, qo[j], minus_one);
+      }
     }
   }
 
@@ -866,19 +898,31 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
         static_for<NB>([&](auto J) {
           constexpr int j = J;
           const u32x4 ko = key_operand<DT, NB>(r.k[u], j);
-          f32x4 t = DT == ELMH_Q4 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc;
+          constexpr bool apart = DT == ELMH_Q4 && !COLS;  // groups' sums, each with its scale
+          f32x4 t = apart ? f32x4{0.f, 0.f, 0.f, 0.f} : sc;
 #pragma unroll
           for (int p = PC - 1; p >= 0; --p) t = mfma<OP>(ko, qo[j][p], t);
-          if constexpr (DT == ELMH_Q4) {
+          if constexpr (apart) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[i] = fmaf(row_bcast<2 * j + u>(r.ks[i]), t[i], sc[i]);
+            for (int i = 0; i < 4; ++i) sc[i] = fmaf(row_bcast<2 * j + u>(r.ks[0][i]), t[i], sc[i]);
           } else {
             sc = t;
           }
         });
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * u + i] = DT == ELMH_Q8 ? sc[i] * (row_bcast<u>(r.ks[i]) * scale) : sc[i] * scale;
+      for (int i = 0; i < 4; ++i) {
+        float v = sc[i];
+        if constexpr (COLS) {  // the same sum in all of a head's lanes: halves, then quarters, ...
+          v *= r.ks[u][i];
+          v += dpp_f<kDppRowRor8>(v);
+          if constexpr (NB >= 4) v += dpp_f<kDppRowRor4>(v);
+          if constexpr (NB >= 8) v += dpp_f<kDppRowRor2>(v);
+        } else if constexpr (DT == ELMH_Q8) {
+          v *= row_bcast<u>(r.ks[0][i]);
+        }
+        s[4 * u + i] = v * scale;
+      }
     });
     const PagedTile now = tile;
     if constexpr (more) {
@@ -892,8 +936,8 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
       for (int i = 0; i < 8; ++i) s[i] = 4 * g + i % 4 < now.valid[i / 4] ? s[i] : -INFINITY;
     }
 
-    const float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    const float mn = fmaxf(m, max_over_groups(top));
+    const float top = max_of(max_of(max_of(max_of(s[0], s[1]), s[2]), max_of(max_of(s[3], s[4]), s[5])), max_of(s[6], s[7]));
+    const float mn = max_of(m, max_over_groups(top));
     const float ref = mn == -INFINITY ? 0.f : mn;  // no token so far: weights of 0, not of exp(-inf + inf)
     float p[8];
 #pragma unroll
@@ -910,11 +954,20 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
           for (int k = 0; k < value_words(DT, NB); ++k) r.v[i][k] = 4 * g + i % 4 < now.valid[i / 4] ? r.v[i][k] : 0u;
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.vs[i] = 4 * g + i < (su ? now.valid[1] : now.valid[0]) ? r.vs[i] : 0.f;
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (COLS) {
+            r.vs[0][i] = 4 * g + i < now.valid[0] ? r.vs[0][i] : 0.f;
+            r.vs[1][i] = 4 * g + i < now.valid[1] ? r.vs[1][i] : 0.f;
+          } else {
+            r.vs[0][i] = 4 * g + i < (su ? now.valid[1] : now.valid[0]) ? r.vs[0][i] : 0.f;
+          }
+        }
       }
     }
     if constexpr (NG > 0) {
-      const float big = fmaxf(fmaxf(fabsf(r.vs[0]), fabsf(r.vs[1])), fmaxf(fabsf(r.vs[2]), fabsf(r.vs[3])));
+      float big = fmaxf(fmaxf(fabsf(r.vs[0][0]), fabsf(r.vs[0][1])), fmaxf(fabsf(r.vs[0][2]), fabsf(r.vs[0][3])));
+      if constexpr (COLS)
+        big = fmaxf(big, fmaxf(fmaxf(fabsf(r.vs[1][0]), fabsf(r.vs[1][1])), fmaxf(fabsf(r.vs[1][2]), fabsf(r.vs[1][3]))));
       if (__any(big > pow2(vexp))) {  // rare after the first tokens
         const int ex = min((int)(__float_as_uint(wave_max(big)) >> 23) - 126, 100);
         fade *= pow2(max(vexp - ex, -126));
@@ -946,15 +999,15 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
 #pragma unroll
           for (int k = 0; k < value_words(DT, NB); ++k) r.v[i][k] ^= 0x80808080u;
       }
-      constexpr int runs = DT == ELMH_Q4 ? NB : 1;  // of values that share their scale
+      constexpr int runs = DT == ELMH_Q4 && !COLS ? NB : 1;  // of values that share their scale
       static_for<runs>([&](auto J) {
         constexpr int j = J;
         u32x4 po[PC];
         float t[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          t[i] = NG ? row_bcast<2 * j>(r.vs[i]) * p[i] : p[i];
-          t[4 + i] = NG ? row_bcast<2 * j + 1>(r.vs[i]) * p[4 + i] : p[4 + i];
+          t[i] = COLS ? r.vs[0][i] * p[i] : NG ? row_bcast<2 * j>(r.vs[0][i]) * p[i] : p[i];
+          t[4 + i] = COLS ? r.vs[COLS][i] * p[4 + i] : NG ? row_bcast<2 * j + 1>(r.vs[0][i]) * p[4 + i] : p[4 + i];
         }
         split8<OP>(t, po, minus_one);
 #pragma unroll
@@ -984,12 +1037,14 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   }
   lds_barrier();  // the queries have been read
   float* stat = lds + kPaWaves * heads * HD;
-  if (n < heads) {
+  if (qn < heads) {
 #pragma unroll
     for (int x = 0; x < 2 * NB; ++x)
+      if (!COLS || x / 2 == sj) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) lds[(wave * heads + n) * HD + value_dim<DT, NB>(x, 4 * g + i)] = acc[x][i];
-    if (g == 0) {
+        for (int i = 0; i < 4; ++i) lds[(wave * heads + qn) * HD + value_dim<DT, NB>(x, 4 * g + i)] = acc[x][i];
+      }
+    if (g == 0 && qn == n) {
       stat[wave * kPaHeads + n] = m;
       stat[(kPaWaves + wave) * kPaHeads + n] = l;
     }
@@ -1075,30 +1130,36 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs 
   }
 }
 
-template <int DT, int NB>
+template <int DT, int NB, bool COLS>
 hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, hipStream_t s) {
   const int heads = a.group < kPaHeads ? a.group : kPaHeads;
   const size_t lds = (size_t)(kPaWaves * heads * 32 * NB + 2 * kPaWaves * kPaHeads) * sizeof(float);
   if (lds > 64 * 1024) {
     static DeviceOnce once;
-    if (!raise_dynamic_lds(once, (const void*)paged_attention_kernel<DT, NB>, 80 * 1024)) return hipErrorInvalidValue;
+    if (!raise_dynamic_lds(once, (const void*)paged_attention_kernel<DT, NB, COLS>, 80 * 1024)) return hipErrorInvalidValue;
   }
   const dim3 grid(a.parts, a.pages.n_kv * a.head_tiles, n_seqs);
-  paged_attention_kernel<DT, NB><<<grid, 64 * kPaWaves, lds, s>>>(a);
+  paged_attention_kernel<DT, NB, COLS><<<grid, 64 * kPaWaves, lds, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
   paged_join_kernel<NB><<<dim3(a.n_heads, n_seqs), kJoinThreads, 0, s>>>(a);
   return hipGetLastError();
 }
+template <int DT, int NB>
+hipError_t launch_paged_attention_cols(const PagedAttnArgs& a, int n_seqs, hipStream_t s) {
+  if constexpr (DT == ELMH_Q4 && (NB == 2 || NB == 4 || NB == 8))
+    if (a.group * NB <= kPaHeads) return launch_paged_attention_as<DT, NB, true>(a, n_seqs, s);
+  return launch_paged_attention_as<DT, NB, false>(a, n_seqs, s);
+}
 template <int DT>
 hipError_t launch_paged_attention_of(const PagedAttnArgs& a, int n_seqs, hipStream_t s) {
   switch (a.pages.head_dim) {
-    case 32: return launch_paged_attention_as<DT, 1>(a, n_seqs, s);
-    case 64: return launch_paged_attention_as<DT, 2>(a, n_seqs, s);
-    case 96: return launch_paged_attention_as<DT, 3>(a, n_seqs, s);
-    case 128: return launch_paged_attention_as<DT, 4>(a, n_seqs, s);
-    case 192: return launch_paged_attention_as<DT, 6>(a, n_seqs, s);
-    case 256: return launch_paged_attention_as<DT, 8>(a, n_seqs, s);
+    case 32: return launch_paged_attention_cols<DT, 1>(a, n_seqs, s);
+    case 64: return launch_paged_attention_cols<DT, 2>(a, n_seqs, s);
+    case 96: return launch_paged_attention_cols<DT, 3>(a, n_seqs, s);
+    case 128: return launch_paged_attention_cols<DT, 4>(a, n_seqs, s);
+    case 192: return launch_paged_attention_cols<DT, 6>(a, n_seqs, s);
+    case 256: return launch_paged_attention_cols<DT, 8>(a, n_seqs, s);
   }
   return hipErrorInvalidValue;
 }

@@ -83,7 +83,7 @@ def _rope(**kw):
 
 @pytest.mark.parametrize("code,kw", [
     (0, {}), (0, dict(dtype=E.F32, k_scale=None, v_scale=None)), (0, dict(dtype=E.BF16)), (0, dict(page_size=4096)), (0, dict(page_size=48)),
-    (0, dict(n_pages=2**31 - 1)),
+    (0, dict(n_pages=2**31 - 1, n_kv=1)), (0, dict(n_pages=2**29 - 1)), (1, dict(n_pages=2**29)), (1, dict(n_pages=2**25, page_size=256)),
     (4, dict(dtype=3)), (4, dict(dtype=-1)), (4, dict(head_dim=80)), (4, dict(head_dim=160)), (4, dict(head_dim=0)), (4, dict(head_dim=512)),
     (1, dict(page_size=8)), (1, dict(page_size=24)), (1, dict(page_size=0)), (1, dict(page_size=8192)), (1, dict(n_kv=0)), (1, dict(n_kv=1025)),
     (1, dict(n_pages=0)), (1, dict(n_pages=2**31)), (1, dict(k=None)), (1, dict(v=None)), (1, dict(k=A + 8)), (1, dict(v=A + 4)),
