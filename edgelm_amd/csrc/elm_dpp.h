@@ -54,4 +54,19 @@ __device__ __forceinline__ int wave_sum_i(int v) {
          __builtin_amdgcn_readlane(v, 48);
 }
 
+// Inclusive sum over the lanes up to each (every lane active): within each 16 lanes (row_shr:1, 2, 4, 8), then the last lane of
+// row 0 and 2 into rows 1 and 3 (row_bcast:15), then lane 31 into the upper half (row_bcast:31).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan_i(int v) {
+  v = scan_step<0x111, 0xF>(v);
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);
+  return scan_step<0x143, 0xC>(v);
+}
+
 }  // namespace elmh

@@ -63,12 +63,46 @@ ELM_HD int64_t kv_page_of(const int32_t* table_row, int max_pages, int64_t n_pag
 
 // ---------------------------------------------------------------- the split of a sequence
 
-// Units of kSplitUnit tokens per part when `units` are split over at most `parts`, each of at least `least`
-ELM_HD int split_size(int units, int parts, int least) {
-  const int per = (units + parts - 1) / parts;
-  return per > least ? per : least;
-}
 ELM_HD int split_parts(int units, int per) { return (units + per - 1) / per; }
+
+constexpr int kPartLeastUnits = 4;   // of a part: one unit a wave
+constexpr int kPartFairUnits = 12;   // a part that is worth its start and end
+constexpr int kPartLongUnits = 64;   // a part whose start and end no longer matter
+constexpr int kPartMostExtra = 1024;
+// Workgroups that are on the card together: as many a CU as the kernel's registers leave room for, one to four
+inline int part_workgroups(int dtype, int head_dim) {
+  return 256 * (head_dim > 128 ? 1 : head_dim <= 64 ? 4 : dtype == ELMH_F32 || dtype == ELMH_BF16 ? 2 : 3);
+}
+// Parts beside one a sequence: three times the workgroups on the card, over the `rows` (kv heads times their tiles) that take
+// every part, but none that a batch of max_len cannot fill
+inline int part_extra(int workgroups, int rows, int n_seqs, int max_len) {
+  const int64_t units = (max_len + kSplitUnit - 1) / kSplitUnit;
+  const int64_t most = (units + kPartLeastUnits - 1) / kPartLeastUnits * n_seqs;
+  int64_t want = 3 * (int64_t)workgroups / rows;
+  if (want < 1) want = 1;
+  if (want > kPartMostExtra) want = kPartMostExtra;
+  return (int)(want < most ? want : most);
+}
+// Parts that `total` is cut into where all of them are to be on the card together, their sequences' shorter last ones counted
+inline int part_once(int workgroups, int rows, int n_seqs, int extra) {
+  const int all = workgroups / rows, left = all - n_seqs > all / 2 ? all - n_seqs : all / 2;
+  return left < 1 ? 1 : left < extra ? left : extra;
+}
+inline int part_few(int rows, int extra) {
+  const int few = 256 / rows;
+  return few < 1 ? 1 : few < extra ? few : extra;
+}
+// Units a part: the batch's `total` over `once`, but of kPartFairUnits as long as `few` parts (one workgroup a CU) are left; where
+// that gives parts of kPartLongUnits and more, over up to `extra`, so that uneven ends even out. (64 q4 sequences of 8 to 16
+// thousand positions, 8 kv heads: 512 workgroups 212 us, 1536 201; one bf16 sequence of 100k: 512 78 us, 1536 85.)
+ELM_HD int part_size(int total, int few, int once, int extra) {
+  const int small = split_parts(total, once), fair = split_parts(total, few), least = split_parts(total, extra);
+  int per = fair < kPartFairUnits ? fair : kPartFairUnits;
+  if (small > per) per = small;
+  if (per > kPartLongUnits) per = kPartLongUnits;
+  if (least > per) per = least;
+  return per > kPartLeastUnits ? per : kPartLeastUnits;
+}
 
 // ---------------------------------------------------------------- what a call has to satisfy
 
@@ -167,10 +201,11 @@ inline PagedFault check_paged_attention(const float* q, const float* out, int64_
   if (q == out) return {ELMH_ERR_ARG, "out may not overlap q"};
   if (n_heads < 1 || n_heads % pages->n_kv || n_heads / pages->n_kv > 256)
     return {ELMH_ERR_ARG, "n_heads: a multiple of the kv heads, at most 256 of each"};
-  if (n_seqs > 65535) return {ELMH_ERR_ARG, "at most 65535 sequences a call"};
+  if (n_seqs > 4096) return {ELMH_ERR_ARG, "at most 4096 sequences a call"};
   if (q_row < 0 || q_row > (int64_t(1) << 40)) return {ELMH_ERR_ARG, "q_row: 0 .. 2^40"};
   if (max_len < 1 || max_len > (int64_t)max_pages * pages->page_size)
     return {ELMH_ERR_ARG, "max_len: 1 .. max_pages * page_size"};
+  if ((int64_t)n_seqs * max_len > int64_t(1) << 35) return {ELMH_ERR_ARG, "n_seqs * max_len past 2^35 positions"};
   if (rope && max_len > rope->max_pos) return {ELMH_ERR_ARG, "max_len past the rotary table"};
   return {};
 }

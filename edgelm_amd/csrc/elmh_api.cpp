@@ -1411,9 +1411,9 @@ int elmh_paged_attention_dev(elmh_ctx* c, const float* q, float* out, int64_t q_
   const PagedFault f = check_paged_attention(q, out, q_row, n_heads, pages, table, n_seqs, max_pages, lens, max_len, rope);
   if (f.code) return fail(c, f.code, "paged_attention: %s", f.what);
   DeviceGuard g(c);
-  const int parts = paged_attention_parts(n_seqs, n_heads, pages->n_kv, max_len);
-  if (const int rc = ensure(c, c->pat, paged_attention_scratch_bytes(n_seqs, n_heads, pages->head_dim, parts))) return rc;
-  HIP_OR_FAIL(c, launch_paged_attention(q, out, q_row, n_heads, *pages, table, n_seqs, max_pages, lens, max_len, rope, parts,
+  const PagedSplit split = paged_attention_split(pages->dtype, n_seqs, n_heads, pages->n_kv, pages->head_dim, max_len);
+  if (const int rc = ensure(c, c->pat, split.part_bytes)) return rc;
+  HIP_OR_FAIL(c, launch_paged_attention(q, out, q_row, n_heads, *pages, table, n_seqs, max_pages, lens, max_len, rope, split,
                                         static_cast<float*>(c->pat.p), c->stream));
   return ELMH_OK;
 }

@@ -222,12 +222,16 @@ hipError_t launch_paged_append(const float* k, const float* v, int n, int64_t ro
 hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t head, const elmh_kv_pages& pages,
                              const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq,
                              hipStream_t s);
-// Parts a sequence is split into at most, and the scratch that the parts need (0 for one part)
-int paged_attention_parts(int n_seqs, int n_heads, int n_kv, int max_len);
-size_t paged_attention_scratch_bytes(int n_seqs, int n_heads, int head_dim, int parts);
+// How the attention splits a batch (part_few, part_once, part_extra), and the bytes of the parts' results (0 where no
+// sequence of max_len is split)
+struct PagedSplit {
+  int few = 1, once = 1, extra = 1;
+  size_t part_bytes = 0;
+};
+PagedSplit paged_attention_split(int dtype, int n_seqs, int n_heads, int n_kv, int head_dim, int max_len);
 hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int n_heads, const elmh_kv_pages& pages,
                                   const int32_t* table, int n_seqs, int max_pages, const int32_t* lens, int max_len,
-                                  const elmh_rope* rope, int parts, float* scratch, hipStream_t s);
+                                  const elmh_rope* rope, const PagedSplit& split, float* parts, hipStream_t s);
 // Test hook: S[t][n][b] for pre-quantized row-major activations.
 hipError_t launch_block_sums(const DevWeight& w, const int8_t* xq, int T, int32_t* S, hipStream_t s);
 

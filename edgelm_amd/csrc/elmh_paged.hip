@@ -446,9 +446,6 @@ __device__ __forceinline__ void static_for(F&& f) {
 
 constexpr int kPaWaves = 4;
 constexpr int kPaHeads = 16;       // query heads a workgroup takes: the columns of a 16 x 16 tile
-constexpr int kPaLeastUnits = 4;   // of a part: one unit a wave
-constexpr int kPaWorkgroups = 512;   // a call is split into
-constexpr int kPaMostParts = 512;    // of a sequence
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // The matrix instructions take 16-bit operands, 32 values deep, or f32 ones, 4 deep. Products are exact in both (f32
@@ -695,9 +692,9 @@ struct PagedAttnArgs {
   int max_len;
   const float *cs, *sn;
   int rot, inter;
-  int parts;      // a sequence is split into at most
-  float* part_o;  // [seq][head][part][head_dim], unnormalized
-  float* part_s;  // [seq][head][part][2]: running maximum (base 2), sum
+  int n_seqs, few, once, extra;  // the split: PagedShare, part_size
+  float* part_o;      // [slot][head][head_dim], unnormalized
+  float* part_s;      // [slot][head][2]: running maximum (base 2), sum
 };
 
 // One instruction for two or three operands (a NaN stays one), where fmaxf first quiets what may be signalling
@@ -710,6 +707,43 @@ __device__ __forceinline__ float max_over_groups(float v) {
   return max_of(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+
+// The batch is split by its own lengths, which every workgroup reads: a part's size is the same for all sequences, and a
+// sequence has as many parts of at most that size as it needs (one if it is empty), so that a long sequence among short ones
+// is no longer on the way than the others. n_seqs + extra slots are always enough.
+struct PagedShare {
+  int seq, len, units;
+  int part, parts, first;  // which of the sequence's, of how many, the first one's slot
+};
+// SEQ: of sequence `want`; else of slot `want`. Uniform (every lane of the wave calls); seq < 0: the slot is no sequence's.
+template <bool SEQ>
+__device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, int want) {
+  const int lane = threadIdx.x & 63;
+  const auto len_of = [&](int i) { return i < a.n_seqs ? min(max(a.lens[i], 0), a.max_len) : 0; };
+  const auto units_of = [&](int len) { return (len + kSplitUnit - 1) / kSplitUnit; };
+  int total = 0;
+  for (int i = 0; i < a.n_seqs; i += 64) total += wave_sum_i(units_of(len_of(i + lane)));
+  const int per = part_size(total, a.few, a.once, a.extra);
+  int before = 0;
+  for (int i = 0; i < a.n_seqs; i += 64) {
+    const int len = len_of(i + lane), units = units_of(len), parts = i + lane < a.n_seqs ? max(1, split_parts(units, per)) : 0;
+    const int sum = wave_scan_i(parts);
+    const uint64_t past = SEQ ? (want < i + 64 ? ~uint64_t(0) << (want - i) : 0) : __ballot(before + sum > want);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      PagedShare s;
+      s.seq = i + at;
+      s.len = __builtin_amdgcn_readlane(len, at);
+      s.units = __builtin_amdgcn_readlane(units, at);
+      s.parts = __builtin_amdgcn_readlane(parts, at);
+      s.first = before + __builtin_amdgcn_readlane(sum, at) - s.parts;
+      s.part = want - s.first;
+      return s;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return {-1, 0, 0, 0, 0, 0};
+}
 
 // Two blocks of 16 tokens (a wave's step): where they lie, and how many tokens of each count (0: behind the end, or no page)
 struct PagedTile {
@@ -742,17 +776,16 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   extern __shared__ float lds[];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int part = blockIdx.x, kvh = blockIdx.y / a.head_tiles, seq = blockIdx.z;
-  const int h0 = kvh * a.group + blockIdx.y % a.head_tiles * kPaHeads;
+  const int kvh = blockIdx.x / a.head_tiles;
+  const int h0 = kvh * a.group + blockIdx.x % a.head_tiles * kPaHeads;
   const int heads = min(kPaHeads, (kvh + 1) * a.group - h0);
   const elmh_kv_pages& pg = a.pages;
-  const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[seq], 0), a.max_len));
-  const int units = (len + kSplitUnit - 1) / kSplitUnit;
-  const int per = split_size(units, a.parts, kPaLeastUnits), live = split_parts(units, per);
+  const PagedShare share = paged_share<false>(a, blockIdx.y);
+  const int seq = share.seq, len = share.len;
+  if (seq < 0) return;
   float* out = a.out + (int64_t)seq * a.n_heads * HD + (int64_t)h0 * HD;
-  if (part >= live) {
-    if (part == 0)  // an empty sequence
-      for (int i = tid; i < heads * HD; i += 64 * kPaWaves) out[i] = 0.f;
+  if (len == 0) {
+    for (int i = tid; i < heads * HD; i += 64 * kPaWaves) out[i] = 0.f;
     return;
   }
 
@@ -813,8 +846,9 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
     load_scales(r.vs, pg.v_scale, t);
   };
 
-  const int end = min(units, (part + 1) * per);
-  int unit = part * per + wave;
+  // at most 2^23 units times kPartMostExtra + 1 parts
+  const int end = (int)((uint32_t)share.units * (uint32_t)(share.part + 1) / (uint32_t)share.parts);
+  int unit = (int)((uint32_t)share.units * (uint32_t)share.part / (uint32_t)share.parts) + wave;
   const bool busy = unit < end;  // a wave without a unit joins with nothing
   int id[2];
   PagedTile tile;
@@ -1063,10 +1097,10 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
       o += f * lds[(w * heads + h) * HD + d];
       L += f * stat[(kPaWaves + w) * kPaHeads + h];
     }
-    if (live == 1) {
+    if (share.parts == 1) {
       out[i] = L == 0.f ? 0.f : o / L;
     } else {
-      const int64_t at = ((int64_t)seq * a.n_heads + h0 + h) * a.parts + part;
+      const int64_t at = (int64_t)blockIdx.y * a.n_heads + h0 + h;
       a.part_o[at * HD + d] = o;
       if (d == 0) {
         a.part_s[at * 2] = M;
@@ -1077,32 +1111,34 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
 }
 
 // The parts of a (sequence, head) joined, always in the same order: the parts' weights first, then their rows, four values a
-// thread, the threads' sums of every (256 / (head_dim / 4))-th part added in turn.
+// thread, the threads' sums of every (256 / (head_dim / 4))-th part added in turn. A launch of its own: joined by the workgroup
+// that ends last, the same parts have to cross from one XCD's L2 to another's, which with a fence takes the whole L2 each
+// time (the 100k-position bf16 case 155 us, so 78), and with loads and stores past the L2 is slower too (88 us; 30k positions
+// of q4 32 us, so 20).
 constexpr int kJoinThreads = 256;
 template <int NB>
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs a) {
   constexpr int HD = 32 * NB, Q = HD / 4, G = kJoinThreads / Q;
-  __shared__ float w[kPaMostParts], wave_m[kJoinThreads / 64], wave_l[kJoinThreads / 64];
+  __shared__ float w[kPartMostExtra + 1], wave_m[kJoinThreads / 64], wave_l[kJoinThreads / 64];
   __shared__ f32x4 sum[G][Q];
   const int tid = threadIdx.x, head = blockIdx.x, seq = blockIdx.y;
-  const int len = min(max(a.lens[seq], 0), a.max_len);
-  const int units = (len + kSplitUnit - 1) / kSplitUnit;
-  const int live = split_parts(units, split_size(units, a.parts, kPaLeastUnits));
-  if (live < 2) return;
-  const int64_t at = ((int64_t)seq * a.n_heads + head) * a.parts;
+  const PagedShare share = paged_share<true>(a, seq);
+  const int parts = share.parts;
+  if (parts < 2) return;
+  const int64_t at = (int64_t)share.first * a.n_heads + head, step = a.n_heads;
   const float* stats = a.part_s + at * 2;
   float M = -INFINITY;
-  for (int s = tid; s < live; s += kJoinThreads) M = fmaxf(M, stats[2 * s]);
+  for (int s = tid; s < parts; s += kJoinThreads) M = fmaxf(M, stats[2 * s * step]);
   M = wave_max(M);
   if ((tid & 63) == 0) wave_m[tid >> 6] = M;
   __syncthreads();
   M = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
   const float ref = M == -INFINITY ? 0.f : M;
   float L = 0.f;
-  for (int s = tid; s < live; s += kJoinThreads) {
-    const float f = __builtin_amdgcn_exp2f(stats[2 * s] - ref);
+  for (int s = tid; s < parts; s += kJoinThreads) {
+    const float f = __builtin_amdgcn_exp2f(stats[2 * s * step] - ref);
     w[s] = f;
-    L += f * stats[2 * s + 1];
+    L += f * stats[2 * s * step + 1];
   }
 #pragma unroll
   for (int off = 32; off; off >>= 1) L += __shfl_xor(L, off, 64);
@@ -1114,8 +1150,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs 
     f32x4 o{0.f, 0.f, 0.f, 0.f};
     const f32x4* rows = reinterpret_cast<const f32x4*>(a.part_o + at * HD) + c;
 #pragma unroll 4
-    for (int s = grp; s < live; s += G) {
-      const f32x4 v = rows[(int64_t)s * Q];
+    for (int s = grp; s < parts; s += G) {
+      const f32x4 v = rows[s * step * Q];
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] += w[s] * v[i];
     }
@@ -1138,10 +1174,10 @@ hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, hipStre
     static DeviceOnce once;
     if (!raise_dynamic_lds(once, (const void*)paged_attention_kernel<DT, NB, COLS>, 80 * 1024)) return hipErrorInvalidValue;
   }
-  const dim3 grid(a.parts, a.pages.n_kv * a.head_tiles, n_seqs);
+  const dim3 grid(a.pages.n_kv * a.head_tiles, n_seqs + a.extra);  // slots of no sequence come last
   paged_attention_kernel<DT, NB, COLS><<<grid, 64 * kPaWaves, lds, s>>>(a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.parts == 1) return e;
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !a.part_o) return e;
   paged_join_kernel<NB><<<dim3(a.n_heads, n_seqs), kJoinThreads, 0, s>>>(a);
   return hipGetLastError();
 }
@@ -1284,21 +1320,20 @@ hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t hea
   return launch_rows(a, rows_aligned(a, k, v), s);
 }
 
-int paged_attention_parts(int n_seqs, int n_heads, int n_kv, int max_len) {
-  const int tiles = (n_heads / n_kv + kPaHeads - 1) / kPaHeads;
-  const int64_t rows = (int64_t)n_seqs * n_kv * tiles;
-  const int units = (max_len + kSplitUnit - 1) / kSplitUnit, most = (units + kPaLeastUnits - 1) / kPaLeastUnits;
-  const int64_t want = std::max<int64_t>(1, kPaWorkgroups / rows);
-  return (int)std::min<int64_t>({want, most, kPaMostParts});
-}
-
-size_t paged_attention_scratch_bytes(int n_seqs, int n_heads, int head_dim, int parts) {
-  return parts > 1 ? (size_t)n_seqs * n_heads * parts * (head_dim + 2) * sizeof(float) : 0;
+PagedSplit paged_attention_split(int dtype, int n_seqs, int n_heads, int n_kv, int head_dim, int max_len) {
+  const int rows = n_kv * ((n_heads / n_kv + kPaHeads - 1) / kPaHeads);
+  PagedSplit p;
+  p.extra = part_extra(part_workgroups(dtype, head_dim), rows, n_seqs, max_len);
+  p.once = part_once(part_workgroups(dtype, head_dim), rows, n_seqs, p.extra);
+  p.few = part_few(rows, p.extra);
+  if (max_len > kPartLeastUnits * kSplitUnit)
+    p.part_bytes = ((size_t)n_seqs + p.extra) * n_heads * (head_dim + 2) * sizeof(float);
+  return p;
 }
 
 hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int n_heads, const elmh_kv_pages& pages,
                                   const int32_t* table, int n_seqs, int max_pages, const int32_t* lens, int max_len,
-                                  const elmh_rope* rope, int parts, float* scratch, hipStream_t s) {
+                                  const elmh_rope* rope, const PagedSplit& split, float* parts, hipStream_t s) {
   PagedAttnArgs a{};
   a.q = q;
   a.out = out;
@@ -1318,9 +1353,14 @@ hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int
     a.inter = rope->interleaved;
   }
   a.magic = page_magic(pages.page_size);
-  a.parts = parts;
-  a.part_o = scratch;
-  a.part_s = scratch + (int64_t)n_seqs * n_heads * parts * pages.head_dim;
+  a.n_seqs = n_seqs;
+  a.few = split.few;
+  a.once = split.once;
+  a.extra = split.extra;
+  if (split.part_bytes) {
+    a.part_o = parts;
+    a.part_s = parts + ((int64_t)n_seqs + split.extra) * n_heads * pages.head_dim;
+  }
   switch (pages.dtype) {
     case ELMH_F32: return launch_paged_attention_of<ELMH_F32>(a, n_seqs, s);
     case ELMH_F16: return launch_paged_attention_of<ELMH_F16>(a, n_seqs, s);

@@ -35,8 +35,11 @@ int table(const float* c, const float* s, int64_t p0, int64_t n, int rot, double
 }
 int64_t page_of(const int32_t* row, int mp, int64_t np, int pos, int ps) { return kv_page_of(row, mp, np, pos, page_magic(ps)); }
 int page_index_of(int pos, int ps) { return page_index(pos, page_magic(ps)); }
-int per(int units, int parts, int least) { return split_size(units, parts, least); }
 int parts_of(int units, int per) { return split_parts(units, per); }
+int extra(int dt, int hd, int rows, int n, int max_len) { return part_extra(part_workgroups(dt, hd), rows, n, max_len); }
+int once(int dt, int hd, int rows, int n, int extra) { return part_once(part_workgroups(dt, hd), rows, n, extra); }
+int few(int rows, int extra) { return part_few(rows, extra); }
+int size(int total, int few, int once, int extra) { return part_size(total, few, once, extra); }
 int kbyte(int d, int hd) { return q4_key_byte(d, hd); }
 int vbyte(int d, int hd) { return q4_value_byte(d, hd); }
 double freq(int rot, double th, const elmh_rope_scaling* sc, int i) {
@@ -121,9 +124,9 @@ ATTN = dict(q=A, out=2 * A, q_row=0, n_heads=32, pages=_pages(), table=A, n_seqs
 
 @pytest.mark.parametrize("code,kw", [
     (0, {}), (0, dict(n_heads=8)), (0, dict(n_heads=8 * 256)), (0, dict(max_len=1)), (0, dict(rope=_rope(max_pos=160))), (0, dict(q_row=5000)),
-    (0, dict(n_seqs=65535)),
+    (0, dict(n_seqs=4096)), (1, dict(n_seqs=4096, max_pages=2**24, max_len=2**24)),
     (1, dict(q=None)), (1, dict(out=None)), (1, dict(out=A)), (1, dict(lens=None)), (1, dict(table=None)), (1, dict(n_heads=0)), (1, dict(n_heads=33)),
-    (1, dict(n_heads=4)), (1, dict(n_heads=8 * 257)), (1, dict(max_len=0)), (1, dict(max_len=161)), (1, dict(n_seqs=0)), (1, dict(n_seqs=65536)),
+    (1, dict(n_heads=4)), (1, dict(n_heads=8 * 257)), (1, dict(max_len=0)), (1, dict(max_len=161)), (1, dict(n_seqs=0)), (1, dict(n_seqs=4097)),
     (1, dict(q_row=-1)), (1, dict(rope=_rope(max_pos=159))), (1, dict(pages=_pages(k=None))), (4, dict(pages=_pages(dtype=7))),
 ])
 def test_attention(host, code, kw):
@@ -184,14 +187,24 @@ def test_page_index_is_the_quotient(host):
             assert host.page_index_of(pos, ps) == pos // ps, (pos, ps)
 
 
-def test_parts_cover_a_sequence(host):
-    for least in (1, 4):
-        for parts in (1, 2, 3, 7, 64, 256):
-            for units in (1, 2, 3, 4, 5, 31, 32, 33, 1000, 4097):
-                per = host.per(units, parts, least)
-                live = host.parts_of(units, per)
-                assert per >= least and 1 <= live <= parts and (live - 1) * per < units <= live * per
-    assert host.parts_of(0, host.per(0, 4, 4)) == 0
+def test_parts_fit_their_slots(host):
+    """Whatever the lengths below the host's bound, the parts of all sequences (one of an empty one) are no more than n_seqs +
+    extra, each is of kPartLeastUnits or more unless its sequence is shorter, and a part's bounds are 32-bit products."""
+    rng = np.random.default_rng(0)
+    for rows, hd, dt in ((1, 64, E.F32), (3, 64, E.Q8), (8, 128, E.BF16), (8, 128, E.Q4), (8, 256, E.F16), (40, 128, E.Q8), (1024, 128, E.F32), (16384, 32, E.Q4)):
+        for n in (1, 2, 7, 64, 65, 300, 4096):
+            for max_len in (1, 31, 128, 129, 4096, 100003, 2**23):
+                extra = host.extra(dt, hd, rows, n, max_len)
+                once = host.once(dt, hd, rows, n, extra)
+                assert 1 <= once <= extra <= 1024
+                top = -(-max_len // 32)
+                for units in (np.full(n, top), rng.integers(0, top + 1, n), np.where(np.arange(n) == n // 2, top, 0), np.zeros(n, int),
+                              np.where(rng.random(n) < 0.5, top, 1)):
+                    per = host.size(int(units.sum()), host.few(rows, extra), once, extra)
+                    parts = np.maximum(1, -(-units // per))
+                    assert per >= 4 and parts.sum() <= n + extra, (rows, n, max_len)
+                    assert parts.max() <= extra + 1 and int(units.max()) * (int(parts.max()) + 1) < 2**32
+                    assert host.parts_of(int(units[0]), per) == -(-int(units[0]) // per)
 
 
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 192, 256])
