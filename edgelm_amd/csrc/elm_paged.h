@@ -66,6 +66,9 @@ ELM_HD int64_t kv_page_of(const int32_t* table_row, int max_pages, int64_t n_pag
 ELM_HD int split_parts(int units, int per) { return (units + per - 1) / per; }
 
 constexpr int kPartLeastUnits = 4;   // of a part: one unit a wave
+constexpr int kPartAloneUnits = 16;  // sequences up to this are not split: the second launch costs more (q8, 200 positions: 8.5 us
+                                     // in one, 11.6 split; 500: 10.7 and 11.5; 1000: 14.4 and 11.5)
+inline int part_least(int max_len) { return max_len <= kPartAloneUnits * kSplitUnit ? kPartAloneUnits : kPartLeastUnits; }
 constexpr int kPartFairUnits = 12;   // a part that is worth its start and end
 constexpr int kPartLongUnits = 64;   // a part whose start and end no longer matter
 constexpr int kPartMostExtra = 1024;
@@ -95,13 +98,13 @@ inline int part_few(int rows, int extra) {
 // Units a part: the batch's `total` over `once`, but of kPartFairUnits as long as `few` parts (one workgroup a CU) are left; where
 // that gives parts of kPartLongUnits and more, over up to `extra`, so that uneven ends even out. (64 q4 sequences of 8 to 16
 // thousand positions, 8 kv heads: 512 workgroups 212 us, 1536 201; one bf16 sequence of 100k: 512 78 us, 1536 85.)
-ELM_HD int part_size(int total, int few, int once, int extra) {
+ELM_HD int part_size(int total, int few, int once, int extra, int at_least) {
   const int small = split_parts(total, once), fair = split_parts(total, few), least = split_parts(total, extra);
   int per = fair < kPartFairUnits ? fair : kPartFairUnits;
   if (small > per) per = small;
   if (per > kPartLongUnits) per = kPartLongUnits;
   if (least > per) per = least;
-  return per > kPartLeastUnits ? per : kPartLeastUnits;
+  return per > at_least ? per : at_least;
 }
 
 // ---------------------------------------------------------------- what a call has to satisfy

@@ -202,16 +202,16 @@ struct RowArgs {
   const int32_t *pos, *seq;
   const float *cs, *sn;
   int max_pos, rot, inter;
-  uint32_t magic;  // page_magic(page_size)
+  uint32_t magic;   // page_magic(page_size)
+  int head_shift;   // a workgroup's rows: of 2^head_shift heads
 };
 
-// Where row i of a call lies in the cache; page < 0: the row is skipped
+// Where a row of a call lies in the cache; page < 0: the row is skipped
 struct RowPlace {
   int64_t page;
   int slot, pos;
 };
-__device__ __forceinline__ RowPlace row_place(const RowArgs& a, int i) {
-  const int pos = a.pos[i], seq = a.seq ? a.seq[i] : i;
+__device__ __forceinline__ RowPlace row_place(const RowArgs& a, int pos, int seq) {
   if (seq < 0 || seq >= a.n_seqs || pos < 0 || (a.cs && pos >= a.max_pos)) return {-1, 0, 0};
   return {kv_page_of(a.table + (int64_t)seq * a.max_pages, a.max_pages, a.pages.n_pages, pos, a.magic),
           pos - page_index(pos, a.magic) * a.pages.page_size, pos};
@@ -229,9 +229,17 @@ __device__ __forceinline__ float rotated(const float* x, int d, const float* cs,
 
 // Rows go by eight lanes each: lane c of them holds values 32 j + 4 c .. + 3 of every 32-value group j, so that eight lanes read
 // or write 128 contiguous bytes of f32 a group, the group's q4 scale is a matter of eight lanes, and its eight 4-bit levels
-// lie in neighbouring bytes. A workgroup: 32 rows of one kv head in one pool (grid: rows, heads, pools).
+// lie in neighbouring bytes. A workgroup: 32 rows in one pool (grid: tokens, heads, pools); of neighbouring heads of a token
+// where those are neighbours outside the cache, in f32 most of what is moved, of one head elsewhere.
 constexpr int kRowLanes = 8;
 constexpr int kRowsPerBlock = 256 / kRowLanes;
+
+__device__ __forceinline__ int row_token(const RowArgs& a) {
+  return (int)blockIdx.x * (kRowsPerBlock >> a.head_shift) + ((int)(threadIdx.x / kRowLanes) >> a.head_shift);
+}
+__device__ __forceinline__ int row_head(const RowArgs& a) {
+  return ((int)blockIdx.y << a.head_shift) + ((int)(threadIdx.x / kRowLanes) & ((1 << a.head_shift) - 1));
+}
 
 // max over a row's eight lanes, in one instruction a step
 __device__ __forceinline__ float row_max8(float v) {
@@ -240,49 +248,89 @@ __device__ __forceinline__ float row_max8(float v) {
   return fmaxf(v, dpp_f<kDppHalfMirror>(v));
 }
 
-// x: 4 * NB values of lane c, NB groups. VEC: 16-byte loads (the host has checked that every one is aligned, and that a lane's
+// A row's values in lane c, and with the half layout those that the rotated ones pair with (read again from L1: they are another
+// lane's, or this one's of another group). VEC: 16-byte loads (the host has checked that every one is aligned, and that a lane's
 // four values are either all rotated or none, with their partners four values too).
 template <int NB, bool VEC>
-__device__ __forceinline__ void load_row(float (&x)[NB][4], const float* src, int c, const float* cs, const float* sn, int half,
-                                         int inter) {
-#pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const int d = 32 * j + 4 * c;
+struct AppendRow {
+  float x[NB][4];
+  f32x4 o[VEC ? NB : 1];
+
+  // what does not depend on the row's position, so that it is on its way while the table is looked up
+  __device__ __forceinline__ void load(const float* src, int c, bool turn, int half, int inter) {
     if constexpr (VEC) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(src + d);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j][e] = v[e];
-    } else {
+      for (int j = 0; j < NB; ++j) {
+        const int d = 32 * j + 4 * c;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(src + d);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j][e] = cs ? rotated(src, d + e, cs, sn, half, inter) : src[d + e];
+        for (int e = 0; e < 4; ++e) x[j][e] = v[e];
+        if (turn && !inter && d < 2 * half) o[j] = *reinterpret_cast<const f32x4*>(src + (d >= half ? d - half : d + half));
+      }
     }
   }
-  if constexpr (VEC) {
-    if (!cs) return;
-    // the partners of the half layout are another lane's, or this one's of another group: read again (they are in L1)
+  // cs, sn: the position's row of the tables, or null
+  __device__ __forceinline__ void rotate(const float* src, int c, const float* cs, const float* sn, int half, int inter) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int d = 32 * j + 4 * c;
-      if (d >= 2 * half) continue;
-      if (inter) {
-        const u32x2 co = *reinterpret_cast<const u32x2*>(cs + d / 2), si = *reinterpret_cast<const u32x2*>(sn + d / 2);
+      if constexpr (!VEC) {
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const float cc = __uint_as_float(co[e / 2]), ss = __uint_as_float(si[e / 2]), u = x[j][e], v = x[j][e + 1];
-          x[j][e] = u * cc - v * ss;
-          x[j][e + 1] = v * cc + u * ss;
-        }
-      } else {
-        const bool second = d >= half;
-        const int i = second ? d - half : d;
-        const f32x4 o = *reinterpret_cast<const f32x4*>(src + (second ? i : d + half));
-        const f32x4 co = *reinterpret_cast<const f32x4*>(cs + i), si = *reinterpret_cast<const f32x4*>(sn + i);
+        for (int e = 0; e < 4; ++e) x[j][e] = cs ? rotated(src, d + e, cs, sn, half, inter) : src[d + e];
+      } else if (cs && d < 2 * half) {
+        if (inter) {
+          const float2 co = *reinterpret_cast<const float2*>(cs + d / 2), si = *reinterpret_cast<const float2*>(sn + d / 2);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float ss = second ? si[e] : -si[e];  // u c - v s = u c + v (-s), to the bit
-          x[j][e] = x[j][e] * co[e] + o[e] * ss;
+          for (int e = 0; e < 4; e += 2) {
+            const float cc = e ? co.y : co.x, ss = e ? si.y : si.x, u = x[j][e], v = x[j][e + 1];
+            x[j][e] = u * cc - v * ss;
+            x[j][e + 1] = v * cc + u * ss;
+          }
+        } else {
+          const bool second = d >= half;
+          const int i = second ? d - half : d;
+          const f32x4 co = *reinterpret_cast<const f32x4*>(cs + i), si = *reinterpret_cast<const f32x4*>(sn + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float ss = second ? si[e] : -si[e];  // u c - v s = u c + v (-s), to the bit
+            x[j][e] = x[j][e] * co[e] + o[j][e] * ss;
+          }
         }
       }
+    }
+  }
+};
+
+// N bytes at a multiple of the largest power of two that divides N
+template <int N>
+__device__ __forceinline__ void store_bytes(uint8_t* p, const uint32_t* w) {
+  constexpr int by = N % 16 == 0 ? 16 : N % 8 == 0 ? 8 : N % 4 == 0 ? 4 : 2;
+#pragma unroll
+  for (int i = 0; i < N; i += by) {
+    if constexpr (by == 16) *reinterpret_cast<u32x4*>(p + i) = u32x4{w[i / 4], w[i / 4 + 1], w[i / 4 + 2], w[i / 4 + 3]};
+    else if constexpr (by == 8) *reinterpret_cast<u32x2*>(p + i) = u32x2{w[i / 4], w[i / 4 + 1]};
+    else if constexpr (by == 4) *reinterpret_cast<uint32_t*>(p + i) = w[i / 4];
+    else *reinterpret_cast<uint16_t*>(p + i) = (uint16_t)(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+  constexpr int by = N % 16 == 0 ? 16 : N % 8 == 0 ? 8 : N % 4 == 0 ? 4 : 2;
+#pragma unroll
+  for (int i = 0; i < N; i += by) {
+    if constexpr (by == 16) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(p + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[i / 4 + k] = v[k];
+    } else if constexpr (by == 8) {
+      const u32x2 v = *reinterpret_cast<const u32x2*>(p + i);
+      w[i / 4] = v[0];
+      w[i / 4 + 1] = v[1];
+    } else if constexpr (by == 4) {
+      w[i / 4] = *reinterpret_cast<const uint32_t*>(p + i);
+    } else {
+      const uint32_t v = *reinterpret_cast<const uint16_t*>(p + i);
+      w[i / 4] = i % 4 ? w[i / 4] | v << 16 : v;
     }
   }
 }
@@ -291,17 +339,20 @@ template <int DT, int NB, bool VEC>
 __global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
   constexpr int HD = 32 * NB;
   const elmh_kv_pages& pg = a.pages;
-  const int t = blockIdx.x * kRowsPerBlock + threadIdx.x / kRowLanes, c = threadIdx.x % kRowLanes, h = blockIdx.y;
+  const int t = row_token(a), c = threadIdx.x % kRowLanes, h = row_head(a);
   const bool keys = blockIdx.z == 0;
   if (t >= a.n) return;  // whole rows: the lanes of a row stay together
-  const RowPlace w = row_place(a, t);
-  if (w.page < 0) return;
   const bool turn = keys && a.cs;
   const int half = a.rot / 2;
+  const float* src = (keys ? a.k : a.v) + t * a.row + h * a.head;
+  const int pos = a.pos[t], seq = a.seq ? a.seq[t] : t;
+  AppendRow<NB, VEC> r;
+  r.load(src, c, turn, half, a.inter);
+  const RowPlace w = row_place(a, pos, seq);
+  if (w.page < 0) return;
   const int64_t at = (int64_t)w.pos * half;
-  float x[NB][4];
-  load_row<NB, VEC>(x, (keys ? a.k : a.v) + t * a.row + h * a.head, c, turn ? a.cs + at : nullptr, turn ? a.sn + at : nullptr,
-                    half, a.inter);
+  r.rotate(src, c, turn ? a.cs + at : nullptr, turn ? a.sn + at : nullptr, half, a.inter);
+  const auto& x = r.x;
   const int64_t row = kv_row(w.page, h, w.slot, pg.n_kv, pg.page_size);
   uint8_t* dst = static_cast<uint8_t*>(keys ? pg.k : pg.v) + row * (DT == ELMH_F32 ? 4 * HD : DT == ELMH_Q8 ? HD : DT == ELMH_Q4 ? HD / 2 : 2 * HD);
   float* scales = keys ? pg.k_scale : pg.v_scale;
@@ -330,7 +381,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       int q[4];
-      elm_q8_group<4>(x[j], div, q);
+      elm_level_group<4, -127, 127>(x[j], div, q);
       *reinterpret_cast<uint32_t*>(dst + 32 * j + 4 * c) =
           (q[0] & 0xFF) | (q[1] & 0xFF) << 8 | (q[2] & 0xFF) << 16 | (uint32_t)(q[3] & 0xFF) << 24;
     }
@@ -347,24 +398,24 @@ __global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
       const uint32_t have = (uint32_t)(__ballot(fabsf(m) == amax) >> (threadIdx.x & 56)) & 0xFFu;
       // no lane has it only if a value is not a number
       const float s = __shfl(m, (threadIdx.x & 56) + (have ? __builtin_ctz(have) : 0), 64) / -8.f, div = s == 0.f ? 1.f : s;
-      uint32_t nib[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float r = x[j][e] / div;
-        nib[e] = (uint32_t)((int)fminf(7.f, fmaxf(-8.f, copysignf(floorf(fabsf(r) + 0.5f), r))) + 8);
-      }
-      b[j] = nib[0] | nib[1] << 4 | nib[2] << 8 | nib[3] << 12;
+      int q[4];
+      elm_level_group<4, -8, 7>(x[j], div, q);
+      b[j] = (uint32_t)(q[0] + 8) | (uint32_t)(q[1] + 8) << 4 | (uint32_t)(q[2] + 8) << 8 | (uint32_t)(q[3] + 8) << 12;
       if (c == 0) scales[kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, NB) + (int64_t)j * pg.page_size] = s;
     }
-    if (keys) {  // [c / 2][j]: words of which this lane has one half
+    if (keys) {  // [c / 2][j]: words of which this lane has one half; the even lane stores them
+      uint32_t o[NB];
 #pragma unroll
-      for (int j = 0; j < NB; ++j) *reinterpret_cast<uint16_t*>(dst + (c / 2) * 4 * NB + 4 * j + 2 * (c % 2)) = (uint16_t)b[j];
+      for (int j = 0; j < NB; ++j) o[j] = b[j] | (uint32_t)dpp_i<kDppQuadXor1>(b[j]) << 16;
+      if (c % 2 == 0) store_bytes<4 * NB>(dst + c / 2 * 4 * NB, o);
     } else {  // [2 c][j], [2 c + 1][j]: all of this lane's bytes are neighbours
+      uint32_t o[(2 * NB + 3) / 4] = {};
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        dst[2 * c * NB + j] = (uint8_t)b[j];
-        dst[(2 * c + 1) * NB + j] = (uint8_t)(b[j] >> 8);
+        o[j / 4] |= (b[j] & 0xFF) << (8 * (j % 4));
+        o[(NB + j) / 4] |= (b[j] >> 8) << (8 * ((NB + j) % 4));
       }
+      store_bytes<2 * NB>(dst + 2 * c * NB, o);
     }
   }
 }
@@ -373,10 +424,10 @@ template <int DT, int NB, bool VEC>
 __global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a) {
   constexpr int HD = 32 * NB;
   const elmh_kv_pages& pg = a.pages;
-  const int t = blockIdx.x * kRowsPerBlock + threadIdx.x / kRowLanes, c = threadIdx.x % kRowLanes, h = blockIdx.y;
+  const int t = row_token(a), c = threadIdx.x % kRowLanes, h = row_head(a);
   const bool keys = blockIdx.z == 0;
   if (t >= a.n) return;
-  const RowPlace w = row_place(a, t);
+  const RowPlace w = row_place(a, a.pos[t], a.seq ? a.seq[t] : t);
   if (w.page < 0) return;
   const int64_t row = kv_row(w.page, h, w.slot, pg.n_kv, pg.page_size);
   const uint8_t* src = static_cast<const uint8_t*>(keys ? pg.k : pg.v) +
@@ -411,10 +462,21 @@ __global__ __launch_bounds__(256) void paged_read_kernel(RowArgs a) {
     }
   } else {
     const float* sc = scales + kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, NB);
+    uint32_t b[NB];  // keys: [c / 2][j], words of which this lane's are one half; values: [2 c][j], [2 c + 1][j]
+    if (keys) {
+      load_bytes<4 * NB>(src + c / 2 * 4 * NB, b);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) b[j] >>= 16 * (c % 2);
+    } else {
+      uint32_t o[(2 * NB + 3) / 4];
+      load_bytes<2 * NB>(src + 2 * c * NB, o);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        b[j] = (o[j / 4] >> (8 * (j % 4)) & 0xFF) | (o[(NB + j) / 4] >> (8 * ((NB + j) % 4)) & 0xFF) << 8;
+    }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const uint32_t u = keys ? *reinterpret_cast<const uint16_t*>(src + (c / 2) * 4 * NB + 4 * j + 2 * (c % 2))
-                              : src[2 * c * NB + j] | (uint32_t)src[(2 * c + 1) * NB + j] << 8;
+      const uint32_t u = b[j];
       const float s = sc[(int64_t)j * pg.page_size];
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[j][e] = (float)((int)(u >> (4 * e) & 15) - 8) * s;
@@ -692,7 +754,7 @@ struct PagedAttnArgs {
   int max_len;
   const float *cs, *sn;
   int rot, inter;
-  int n_seqs, few, once, extra;  // the split: PagedShare, part_size
+  int n_seqs, few, once, extra, least;  // the split: PagedShare, part_size
   float* part_o;      // [slot][head][head_dim], unnormalized
   float* part_s;      // [slot][head][2]: running maximum (base 2), sum
 };
@@ -723,7 +785,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, int wa
   const auto units_of = [&](int len) { return (len + kSplitUnit - 1) / kSplitUnit; };
   int total = 0;
   for (int i = 0; i < a.n_seqs; i += 64) total += wave_sum_i(units_of(len_of(i + lane)));
-  const int per = part_size(total, a.few, a.once, a.extra);
+  const int per = part_size(total, a.few, a.once, a.extra, a.least);
   int before = 0;
   for (int i = 0; i < a.n_seqs; i += 64) {
     const int len = len_of(i + lane), units = units_of(len), parts = i + lane < a.n_seqs ? max(1, split_parts(units, per)) : 0;
@@ -1214,6 +1276,8 @@ RowArgs row_args(int n, int64_t row, int64_t head, const elmh_kv_pages& pages, c
   a.pos = pos;
   a.seq = seq;
   a.magic = page_magic(pages.page_size);
+  if (a.head < a.row)
+    while (a.head_shift < 5 && pages.n_kv % (2 << a.head_shift) == 0) ++a.head_shift;
   if (rope) {
     a.cs = rope->cos;
     a.sn = rope->sin;
@@ -1225,7 +1289,8 @@ RowArgs row_args(int n, int64_t row, int64_t head, const elmh_kv_pages& pages, c
 }
 template <int DT, int NB>
 void launch_rows_as(const RowArgs& a, bool vec, hipStream_t s) {
-  const dim3 grid((a.n + kRowsPerBlock - 1) / kRowsPerBlock, a.pages.n_kv, 2);
+  const int tokens = kRowsPerBlock >> a.head_shift;
+  const dim3 grid((a.n + tokens - 1) / tokens, a.pages.n_kv >> a.head_shift, 2);
   if (a.ko) {
     if (vec) paged_read_kernel<DT, NB, true><<<grid, 256, 0, s>>>(a);
     else paged_read_kernel<DT, NB, false><<<grid, 256, 0, s>>>(a);
@@ -1326,7 +1391,8 @@ PagedSplit paged_attention_split(int dtype, int n_seqs, int n_heads, int n_kv, i
   p.extra = part_extra(part_workgroups(dtype, head_dim), rows, n_seqs, max_len);
   p.once = part_once(part_workgroups(dtype, head_dim), rows, n_seqs, p.extra);
   p.few = part_few(rows, p.extra);
-  if (max_len > kPartLeastUnits * kSplitUnit)
+  p.least = part_least(max_len);
+  if (max_len > p.least * kSplitUnit)
     p.part_bytes = ((size_t)n_seqs + p.extra) * n_heads * (head_dim + 2) * sizeof(float);
   return p;
 }
@@ -1355,6 +1421,7 @@ hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int
   a.magic = page_magic(pages.page_size);
   a.n_seqs = n_seqs;
   a.few = split.few;
+  a.least = split.least;
   a.once = split.once;
   a.extra = split.extra;
   if (split.part_bytes) {

@@ -39,7 +39,8 @@ int parts_of(int units, int per) { return split_parts(units, per); }
 int extra(int dt, int hd, int rows, int n, int max_len) { return part_extra(part_workgroups(dt, hd), rows, n, max_len); }
 int once(int dt, int hd, int rows, int n, int extra) { return part_once(part_workgroups(dt, hd), rows, n, extra); }
 int few(int rows, int extra) { return part_few(rows, extra); }
-int size(int total, int few, int once, int extra) { return part_size(total, few, once, extra); }
+int least(int max_len) { return part_least(max_len); }
+int size(int total, int few, int once, int extra, int least) { return part_size(total, few, once, extra, least); }
 int kbyte(int d, int hd) { return q4_key_byte(d, hd); }
 int vbyte(int d, int hd) { return q4_value_byte(d, hd); }
 double freq(int rot, double th, const elmh_rope_scaling* sc, int i) {
@@ -200,9 +201,10 @@ def test_parts_fit_their_slots(host):
                 top = -(-max_len // 32)
                 for units in (np.full(n, top), rng.integers(0, top + 1, n), np.where(np.arange(n) == n // 2, top, 0), np.zeros(n, int),
                               np.where(rng.random(n) < 0.5, top, 1)):
-                    per = host.size(int(units.sum()), host.few(rows, extra), once, extra)
+                    per = host.size(int(units.sum()), host.few(rows, extra), once, extra, host.least(max_len))
                     parts = np.maximum(1, -(-units // per))
                     assert per >= 4 and parts.sum() <= n + extra, (rows, n, max_len)
+                    assert max_len > 512 or parts.max() == 1
                     assert parts.max() <= extra + 1 and int(units.max()) * (int(parts.max()) + 1) < 2**32
                     assert host.parts_of(int(units[0]), per) == -(-int(units[0]) // per)
 
