@@ -757,6 +757,7 @@ struct PagedAttnArgs {
   int n_seqs, few, once, extra, least;  // the split: PagedShare, part_size
   float* part_o;      // [slot][head][head_dim], unnormalized
   float* part_s;      // [slot][head][2]: running maximum (base 2), sum
+  int2* joins;        // [seq]: first slot, parts; null where no sequence is split
 };
 
 // One instruction for two or three operands (a NaN stays one), where fmaxf first quiets what may be signalling
@@ -777,9 +778,8 @@ struct PagedShare {
   int seq, len, units;
   int part, parts, first;  // which of the sequence's, of how many, the first one's slot
 };
-// SEQ: of sequence `want`; else of slot `want`. Uniform (every lane of the wave calls); seq < 0: the slot is no sequence's.
-template <bool SEQ>
-__device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, int want) {
+// The share of a slot. Uniform (every lane of the wave calls); seq < 0: the slot is no sequence's.
+__device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, int slot) {
   const int lane = threadIdx.x & 63;
   const auto len_of = [&](int i) { return i < a.n_seqs ? min(max(a.lens[i], 0), a.max_len) : 0; };
   const auto units_of = [&](int len) { return (len + kSplitUnit - 1) / kSplitUnit; };
@@ -790,7 +790,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, int wa
   for (int i = 0; i < a.n_seqs; i += 64) {
     const int len = len_of(i + lane), units = units_of(len), parts = i + lane < a.n_seqs ? max(1, split_parts(units, per)) : 0;
     const int sum = wave_scan_i(parts);
-    const uint64_t past = SEQ ? (want < i + 64 ? ~uint64_t(0) << (want - i) : 0) : __ballot(before + sum > want);
+    const uint64_t past = __ballot(before + sum > slot);
     if (past) {
       const int at = __builtin_ctzll(past);
       PagedShare s;
@@ -799,7 +799,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, int wa
       s.units = __builtin_amdgcn_readlane(units, at);
       s.parts = __builtin_amdgcn_readlane(parts, at);
       s.first = before + __builtin_amdgcn_readlane(sum, at) - s.parts;
-      s.part = want - s.first;
+      s.part = slot - s.first;
       return s;
     }
     before += __builtin_amdgcn_readlane(sum, 63);
@@ -842,12 +842,17 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   const int h0 = kvh * a.group + blockIdx.x % a.head_tiles * kPaHeads;
   const int heads = min(kPaHeads, (kvh + 1) * a.group - h0);
   const elmh_kv_pages& pg = a.pages;
-  const PagedShare share = paged_share<false>(a, blockIdx.y);
+  const PagedShare share = paged_share(a, blockIdx.y);
   const int seq = share.seq, len = share.len;
   if (seq < 0) return;
   float* out = a.out + (int64_t)seq * a.n_heads * HD + (int64_t)h0 * HD;
+  // for the join (written last: a store ahead of the table's loads would keep them off the scalar cache)
+  const auto note = [&] {
+    if (share.part == 0 && blockIdx.x == 0 && tid == 0 && a.joins) a.joins[seq] = make_int2(share.first, share.parts);
+  };
   if (len == 0) {
     for (int i = tid; i < heads * HD; i += 64 * kPaWaves) out[i] = 0.f;
+    note();
     return;
   }
 
@@ -1170,56 +1175,69 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
       }
     }
   }
+  note();
 }
 
-// The parts of a (sequence, head) joined, always in the same order: the parts' weights first, then their rows, four values a
-// thread, the threads' sums of every (256 / (head_dim / 4))-th part added in turn. A launch of its own: joined by the workgroup
-// that ends last, the same parts have to cross from one XCD's L2 to another's, which with a fence takes the whole L2 each
-// time (the 100k-position bf16 case 155 us, so 78), and with loads and stores past the L2 is slower too (88 us; 30k positions
-// of q4 32 us, so 20).
+// The parts of a (sequence, head) joined, always in the same order: the parts' weights 2^(m - M) first, then their rows, four
+// values a thread, the threads' sums of every (256 / (head_dim / 4))-th part added in turn. Bound by latency, so a thread's
+// first rows are asked for before the weights. A launch of its own: joined by the workgroup that ends last, the same parts have
+// to cross from one XCD's L2 to another's, which with a fence takes the whole L2 each time (the 100k-position bf16 case 155 us,
+// so 78), and with loads and stores past the L2 is slower too (88 us; 30k positions of q4 32 us, so 20).
 constexpr int kJoinThreads = 256;
+constexpr int kJoinAhead = 8;
 template <int NB>
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs a) {
   constexpr int HD = 32 * NB, Q = HD / 4, G = kJoinThreads / Q;
   __shared__ float w[kPartMostExtra + 1], wave_m[kJoinThreads / 64], wave_l[kJoinThreads / 64];
   __shared__ f32x4 sum[G][Q];
   const int tid = threadIdx.x, head = blockIdx.x, seq = blockIdx.y;
-  const PagedShare share = paged_share<true>(a, seq);
-  const int parts = share.parts;
+  const int2 join = a.joins[seq];
+  const int parts = join.y;
   if (parts < 2) return;
-  const int64_t at = (int64_t)share.first * a.n_heads + head, step = a.n_heads;
-  const float* stats = a.part_s + at * 2;
+  const int64_t at = (int64_t)join.x * a.n_heads + head, step = a.n_heads;
+  const int c = tid % Q, grp = tid / Q;
+  const f32x4* rows = reinterpret_cast<const f32x4*>(a.part_o + at * HD) + c;
+  f32x4 v[kJoinAhead];
+#pragma unroll
+  for (int i = 0; i < kJoinAhead; ++i) v[i] = rows[min(grp + i * G, parts - 1) * step * Q];
+  const float2* stats = reinterpret_cast<const float2*>(a.part_s) + at;
   float M = -INFINITY;
-  for (int s = tid; s < parts; s += kJoinThreads) M = fmaxf(M, stats[2 * s * step]);
+  for (int s = tid; s < parts; s += kJoinThreads) M = fmaxf(M, stats[s * step].x);
   M = wave_max(M);
   if ((tid & 63) == 0) wave_m[tid >> 6] = M;
-  __syncthreads();
+  lds_barrier();
   M = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
   const float ref = M == -INFINITY ? 0.f : M;
   float L = 0.f;
   for (int s = tid; s < parts; s += kJoinThreads) {
-    const float f = __builtin_amdgcn_exp2f(stats[2 * s * step] - ref);
+    const float2 st = stats[s * step];
+    const float f = __builtin_amdgcn_exp2f(st.x - ref);
     w[s] = f;
-    L += f * stats[2 * s * step + 1];
+    L += f * st.y;
   }
 #pragma unroll
   for (int off = 32; off; off >>= 1) L += __shfl_xor(L, off, 64);
   if ((tid & 63) == 0) wave_l[tid >> 6] = L;
-  __syncthreads();
+  lds_barrier();
   L = (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]);
-  const int c = tid % Q, grp = tid / Q;
   if (grp < G) {
     f32x4 o{0.f, 0.f, 0.f, 0.f};
-    const f32x4* rows = reinterpret_cast<const f32x4*>(a.part_o + at * HD) + c;
-#pragma unroll 4
-    for (int s = grp; s < parts; s += G) {
-      const f32x4 v = rows[s * step * Q];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += w[s] * v[i];
+    for (int i = 0; i < kJoinAhead; ++i) {
+      const int s = grp + i * G;
+      const float f = s < parts ? w[s] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] += s < parts ? f * v[i][k] : 0.f;
+    }
+#pragma unroll 4
+    for (int s = grp + kJoinAhead * G; s < parts; s += G) {
+      const f32x4 u = rows[s * step * Q];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] += w[s] * u[k];
     }
     sum[grp][c] = o;
   }
-  __syncthreads();
+  lds_barrier();
   if (tid < HD) {
     float o = 0.f;
 #pragma unroll
@@ -1393,7 +1411,7 @@ PagedSplit paged_attention_split(int dtype, int n_seqs, int n_heads, int n_kv, i
   p.few = part_few(rows, p.extra);
   p.least = part_least(max_len);
   if (max_len > p.least * kSplitUnit)
-    p.part_bytes = ((size_t)n_seqs + p.extra) * n_heads * (head_dim + 2) * sizeof(float);
+    p.part_bytes = ((size_t)n_seqs + p.extra) * n_heads * (head_dim + 2) * sizeof(float) + n_seqs * sizeof(int2);
   return p;
 }
 
@@ -1427,6 +1445,7 @@ hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int
   if (split.part_bytes) {
     a.part_o = parts;
     a.part_s = parts + ((int64_t)n_seqs + split.extra) * n_heads * pages.head_dim;
+    a.joins = reinterpret_cast<int2*>(a.part_s + ((int64_t)n_seqs + split.extra) * n_heads * 2);
   }
   switch (pages.dtype) {
     case ELMH_F32: return launch_paged_attention_of<ELMH_F32>(a, n_seqs, s);
