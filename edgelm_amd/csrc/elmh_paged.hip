@@ -25,32 +25,34 @@ using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 // ---------------------------------------------------------------- rotary tables and rotation
 
-// sin and cos of a in f64, to some 2^-44: a less its nearest multiple of pi / 2 (in two parts, so that nothing is lost up to 2^31
-// turns), then the Taylor sums to r^13 and r^14 on [-pi/4, pi/4] (the first terms left out are under 2^-45). The result is
-// rounded to f32, which needs no more; a library sine in f64 costs three times the instructions.
-__device__ __forceinline__ void sincos_f64(double a, double& sn, double& cs) {
-  const double k = rint(a * 0.63661977236758134308);
+// m sin(a) and m cos(a) rounded to f32: a (in f64, |a| < 2^31) less its nearest multiple k of pi / 2, which adding 1.5 2^52 leaves
+// in the low bits (pi / 2 in two parts, so that nothing is lost), then the Taylor sums to r^11 and r^12 on [-pi / 4, pi / 4]: the
+// first terms left out are under 2^-36, a four-thousandth of a half step. Some 32 instructions; a library sine in f64 takes
+// five times as many.
+__device__ __forceinline__ void sincos_f64(double a, double m, float& sn, float& cs) {
+  constexpr double kShift = 6755399441055744.0;
+  const double t = fma(a, 0.63661977236758134308, kShift);
+  const uint32_t q = (uint32_t)__double_as_longlong(t);
+  const double k = t - kShift;
   double r = fma(k, -1.57079632679489655800, a);
   r = fma(k, -6.12323399573676603587e-17, r);
   const double z = r * r;
-  double s = fma(z, 1.0 / 6227020800, -1.0 / 39916800);
-  s = fma(s, z, 1.0 / 362880);
+  double s = fma(z, -1.0 / 39916800, 1.0 / 362880);
   s = fma(s, z, -1.0 / 5040);
   s = fma(s, z, 1.0 / 120);
   s = fma(s, z, -1.0 / 6);
-  s = fma(s * z, r, r);
-  double c = fma(z, -1.0 / 87178291200, 1.0 / 479001600);
-  c = fma(c, z, -1.0 / 3628800);
+  const double rm = r * m;
+  s = fma(s * z, rm, rm);
+  double c = fma(z, 1.0 / 479001600, -1.0 / 3628800);
   c = fma(c, z, 1.0 / 40320);
   c = fma(c, z, -1.0 / 720);
   c = fma(c, z, 1.0 / 24);
   c = fma(c, z, -0.5);
-  c = fma(c, z, 1.0);
-  const int q = (int)k;  // a position under 2^31 at a frequency of at most 1: |k| < 2^31
+  c = fma(c, z * m, m);
+  const float fs = (float)s, fc = (float)c;
   const bool swap = q & 1;
-  const double u = swap ? c : s, v = swap ? s : c;
-  sn = q & 2 ? -u : u;
-  cs = (q + 1) & 2 ? -v : v;
+  sn = __uint_as_float(__float_as_uint(swap ? fc : fs) ^ ((q & 2) << 30));
+  cs = __uint_as_float(__float_as_uint(swap ? fs : fc) ^ (((q + 1) & 2) << 30));
 }
 
 // Workgroups of whole rows (positions): each takes the pairs' frequencies into LDS once (a power in f64 costs as much as many
@@ -71,10 +73,7 @@ __global__ __launch_bounds__(256) void rope_table_kernel(float* __restrict__ cs,
     float c[W], s[W];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      double u, v;
-      sincos_f64(p * freq[W * col + w], u, v);
-      s[w] = (float)(u * band.magnitude);
-      c[w] = (float)(v * band.magnitude);
+      sincos_f64(p * freq[W * col + w], band.magnitude, s[w], c[w]);
     }
     const int64_t at = (first + row) * half + W * col;
     if constexpr (W == 4) {
