@@ -169,7 +169,7 @@ inline RowStrides row_strides(int64_t row, int64_t head, int n_kv, int head_dim)
 }
 // written: the rows go to memory, so no two of them may share a value
 inline PagedFault check_rows(int64_t n, int64_t row, int64_t head, int n_kv, int head_dim, bool written) {
-  if (n < 1 || n > (int64_t(1) << 24)) return {ELMH_ERR_ARG, "rows outside 1 .. 2^24"};
+  if (n < 1 || n > 1 << 23) return {ELMH_ERR_ARG, "rows outside 1 .. 2^23"};
   constexpr int64_t most = int64_t(1) << 40;
   if (row < 0 || head < 0 || row > most || head > most) return {ELMH_ERR_ARG, "row and head strides: 0 .. 2^40"};
   const RowStrides s = row_strides(row, head, n_kv, head_dim);

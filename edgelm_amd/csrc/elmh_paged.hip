@@ -954,7 +954,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
 #pragma unroll
         for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qrow[32 * j + 8 * g + e]));
       big = max_over_groups(big);  // (with COLS every lane of a head reads all of its groups)
-      const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 100);
+      const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 127);
       up = pow2(9 - ex);
       scale *= pow2(ex - 9 + (NG ? kLevelExp : 0));
     }
@@ -1069,7 +1069,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
       if constexpr (COLS)
         big = fmaxf(big, fmaxf(fmaxf(fabsf(r.vs[1][0]), fabsf(r.vs[1][1])), fmaxf(fabsf(r.vs[1][2]), fabsf(r.vs[1][3]))));
       if (__any(big > pow2(vexp))) {  // rare after the first tokens
-        const int ex = min((int)(__float_as_uint(wave_max(big)) >> 23) - 126, 100);
+        const int ex = min((int)(__float_as_uint(wave_max(big)) >> 23) - 126, 127);
         fade *= pow2(max(vexp - ex, -126));
         vexp = ex;
       }
@@ -1352,7 +1352,7 @@ hipError_t launch_rope_table(float* cs, float* sn, int64_t pos0, int64_t n, int 
   const int64_t one = std::max<int64_t>(1, 256 / (wide ? half / 4 : half));
   const int64_t rows = one * std::min<int64_t>(16, std::max<int64_t>(1, n / (one * 2048)));
   const int64_t blocks = (n + rows - 1) / rows;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  if (blocks >= 1 << 24) return hipErrorInvalidValue;  // of 256 threads; more table than the card holds
   if (wide)
     rope_table_kernel<4><<<(unsigned)blocks, 256, 0, s>>>(cs, sn, pos0, n, half, (int)rows, theta, band);
   else

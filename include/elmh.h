@@ -261,7 +261,7 @@ int elmh_argmax_step_dev(elmh_ctx* ctx, const float* x, int64_t n, int32_t* out,
  * are NULL for the float types) and the page table [n_seqs][max_pages]: position p of sequence s is slot p % page_size of page
  * table[s][p / page_size]. Entries outside 0 .. n_pages - 1 name no page: nothing is read or written through them. One page may
  * be in several sequences (a shared prefix); a position is written at most once a call (written twice, its row is
- * unspecified). */
+ * unspecified). Limits: 1024 kv heads, pages of 4096 and sequences of 2^28 positions, 2^23 rows a call of append and read. */
 typedef struct {
   int dtype, n_kv, head_dim, page_size;
   int64_t n_pages;
@@ -316,6 +316,7 @@ int elmh_paged_read_dev(elmh_ctx* ctx, float* k, float* v, int n, int64_t row, i
  * n_heads * head_dim], not overlapping q. lens is read on the device and bounded to 0 .. max_len; max_len, the host's bound,
  * sizes the launch. A sequence of length 0 (padding) gives zeros; positions of no page are left out; slots behind a sequence's
  * end may hold anything. Products and sums in f32 or as exact as it (quantized levels are multiplied as they are).
+ * At most 4096 sequences, 256 query heads a kv head, and n_seqs * max_len of 2^35.
  * Long sequences are split over workgroups and joined, in a device buffer the context allocates and grows outside capture
  * (elmh_scratch_generation); results do not depend on the order in which the parts end. */
 int elmh_paged_attention_dev(elmh_ctx* ctx, const float* q, float* out, int64_t q_row, int n_heads,

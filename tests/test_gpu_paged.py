@@ -351,6 +351,60 @@ def test_attention_of_uneven_scales(ctx, dtype):
     c.free()
 
 
+@pytest.mark.parametrize("dtype", ["q8", "q4", "f32", "bf16"])
+@pytest.mark.parametrize("k_amp,v_amp,q_amp", [(1e-30, 1e34, 1e30), (1e30, 1e-34, 1e-30)])
+def test_attention_at_the_ends_of_the_range(ctx, dtype, k_amp, v_amp, q_amp):
+    """Values and queries near the largest and smallest f32 holds, under keys that bring the scores back."""
+    rng = np.random.default_rng(15)
+    lens, page, n_kv, hd = [100, 33], 16, 2, 64
+    table = _table_of(rng, lens, page, 12)
+    c = Cache(ctx, dtype, n_kv, hd, page, 12)
+    _fill(c, rng, table, lens, k_amp, v_amp)
+    c.send()
+    q = rng.normal(0, q_amp, (2, 4, hd)).astype(np.float32)
+    want, tol = _attention64(c, q, table, lens)
+    _check(_attend(ctx, c, q, table, lens) * 1.0, want, tol)
+    c.free()
+
+
+@pytest.mark.parametrize("dtype,hd", [("q8", 64), ("q4", 64), ("bf16", 128)])
+def test_attention_of_many_sequences(ctx, dtype, hd):
+    """More sequences than a wave has lanes, most of them short or empty, a few long ones that are split, at either end and
+    between; and batches of 64 and 65. Pages shared by many sequences."""
+    rng = np.random.default_rng(17)
+    page, n_kv, n_pages = 16, 1, 12
+    c = Cache(ctx, dtype, n_kv, hd, page, n_pages)
+    for p in range(n_pages):
+        for s in range(page):
+            c.put("k", p, 0, s, rng.normal(0, 1, hd))
+            c.put("v", p, 0, s, rng.normal(0, 1, hd))
+    c.send()
+    rows = {(n, p): np.stack([c.get(n, p, 0, s) for s in range(page)]) for n in "kv" for p in range(n_pages)}
+    for n in (64, 65, 300):
+        lens = rng.integers(0, 60, n)
+        lens[rng.random(n) < 0.3] = 0
+        lens[[0, n // 2, n - 1]] = [3000, 1700, 2500]
+        table = rng.integers(0, n_pages, (n, 190)).astype(np.int32)
+        q = rng.normal(0, 1, (n, 2, hd)).astype(np.float32)
+        got = _attend(ctx, c, q, table, lens)
+        for b in range(n):
+            if not lens[b]:
+                assert not got[b].any()
+                continue
+            k, v = (np.concatenate([rows[m, p] for p in table[b, :-(-lens[b] // page)]])[:lens[b]] for m in "kv")
+            for i in range(2):
+                s = k @ q[b, i].astype(np.float64) / math.sqrt(hd)
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                o = w @ v
+                # as _attention64's
+                amp = np.sqrt(((k * q[b, i]) ** 2).sum(1) / hd).max() + np.abs(s).max()
+                spread = np.sqrt(w @ ((v - o) ** 2).sum(1))
+                tol = EPS * (8 * math.sqrt(hd) * max(1.0, amp) * (spread + np.linalg.norm(o)) + (math.sqrt(lens[b]) + 8) * np.linalg.norm(o))
+                assert np.linalg.norm(got[b, i] - o) <= tol, (n, b, i)
+    c.free()
+
+
 def test_attention_past_4_gb(ctx):
     """Pages far into pools of more than 4 GB (2^32 bytes, and 2^31 values in f16): addresses are 64-bit."""
     page, n_kv, hd, n_pages, lens = 128, 8, 256, 8400, [200, 129]
@@ -497,8 +551,44 @@ def test_append_and_read_strides(ctx, dtype, order):
     rope.free()
 
 
-def test_append_one_row_to_many(ctx):
-    """One input row for every token (stride past nothing but itself is refused only for outputs) and pages shared by sequences."""
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n_kv,hd,page", [(1, 96, 4096), (5, 32, 16), (8, 128, 48), (12, 64, 80), (64, 32, 16)])
+@pytest.mark.parametrize("off", [0, 1])
+def test_append_and_read_heads(ctx, dtype, n_kv, hd, page, off):
+    """Kv heads that go to one workgroup in powers of two and not, page sizes that are no power of two and the largest, row i of
+    sequence i, rotary tables on and off 16 bytes."""
+    rng = np.random.default_rng([n_kv, hd])
+    n, max_pos = 37, 9000
+    cos, sin = _tables(max_pos, hd)
+    cb, sb = _up(ctx, *[np.concatenate([np.full(off, 9, np.float32), t.ravel()]) for t in (cos, sin)])
+    rope = E.Rope(cb.ptr + 4 * off, sb.ptr + 4 * off, max_pos, hd, 0)
+    r = RopeTables.__new__(RopeTables)
+    r.cos, r.sin, r.rot, r.inter = cos, sin, hd, False
+    pos = rng.integers(0, min(max_pos, 2 * page), n).astype(np.int32)
+    table = rng.permutation(2 * n).reshape(n, 2).astype(np.int32)
+    c = Cache(ctx, dtype, n_kv, hd, page, 2 * n, fill=0).send()
+    k, v = (rng.normal(0, 1, (n, n_kv, hd)).astype(np.float32) for _ in range(2))
+    for i in range(n):
+        for h in range(n_kv):
+            c.put("k", table[i, pos[i] // page], h, pos[i] % page, r.turn(k[i, h], pos[i]))
+            c.put("v", table[i, pos[i] // page], h, pos[i] % page, v[i, h])
+    kb, vb, tb, pb = _up(ctx, k, v, table, pos)
+    ctx.paged_append_dev(kb.ptr, vb.ptr, n, c.pages, tb.ptr, n, 2, pb.ptr, None, rope)
+    pool, scale = c.fetch()
+    for m in "kv":
+        assert np.array_equal(pool[m], c.pool[m])
+        if scale:
+            assert np.array_equal(scale[m], c.scale[m], equal_nan=True)
+    ctx.paged_read_dev(kb.ptr, vb.ptr, n, c.pages, tb.ptr, n, 2, pb.ptr)
+    for b, m in ((kb, "k"), (vb, "v")):
+        got = b.download(k.shape, np.float32)
+        assert all(np.array_equal(got[i, h], c.get(m, table[i, pos[i] // page], h, pos[i] % page).astype(np.float32)) for i in range(n) for h in range(n_kv))
+    _free(kb, vb, tb, pb, cb, sb)
+    c.free()
+
+
+def test_append_to_shared_pages(ctx):
+    """One page in two sequences' rows of the table."""
     n_kv, hd, page = 2, 32, 16
     c = Cache(ctx, "q8", n_kv, hd, page, 2, fill=0).send()
     x = np.random.default_rng(1).normal(0, 1, (n_kv, hd)).astype(np.float32)
@@ -508,12 +598,11 @@ def test_append_one_row_to_many(ctx):
         for h in range(n_kv):
             for m in "kv":
                 c.put(m, table[s, 0], h, p, x[h])
-    xb, tb, pb, zb = _up(ctx, np.stack([x] * 1), table, pos, np.zeros((3, n_kv, hd), np.float32))
-    for i in range(3):  # one call a row: a contiguous row stride of 0 means the default
-        ctx.paged_append_dev(xb.ptr, xb.ptr, 1, c.pages, tb.ptr + 4 * i, 1, 1, pb.ptr + 4 * i)
+    xb, tb, pb = _up(ctx, np.stack([x] * 3), table, pos)
+    ctx.paged_append_dev(xb.ptr, xb.ptr, 3, c.pages, tb.ptr, 3, 1, pb.ptr)
     pool, scale = c.fetch()
     assert all(np.array_equal(pool[m], c.pool[m]) and np.array_equal(scale[m], c.scale[m], equal_nan=True) for m in "kv")
-    _free(xb, tb, pb, zb)
+    _free(xb, tb, pb)
     c.free()
 
 
@@ -544,6 +633,24 @@ def test_rope(ctx, hd, rot, inter, T, heads):
     assert np.array_equal(got[:, :heads * hd], want)
     assert (got[:-1, heads * hd:] == 5).all()
     _free(xb, pb, yb, wb, zb)
+    r.free()
+
+
+@pytest.mark.parametrize("rot", [64, 62])
+def test_rope_of_many_rows(ctx, rot):
+    """More rows than one launch has threads for at once."""
+    T, heads, hd = 17003, 32, 64
+    rng = np.random.default_rng(rot)
+    r = RopeTables(ctx, 700, rot, False)
+    x = rng.normal(0, 1, (T, heads, hd)).astype(np.float32)
+    pos = rng.integers(0, 700, T).astype(np.int32)
+    xb, pb = _up(ctx, x, pos)
+    ctx.rope_dev(xb.ptr, xb.ptr, T, heads, hd, r.rope, pb.ptr)
+    want, half = x.copy(), rot // 2
+    c, s = r.cos[pos][:, None], r.sin[pos][:, None]
+    want[..., :half], want[..., half:rot] = x[..., :half] * c - x[..., half:rot] * s, x[..., half:rot] * c + x[..., :half] * s
+    assert np.array_equal(xb.download(x.shape, np.float32), want)
+    _free(xb, pb)
     r.free()
 
 

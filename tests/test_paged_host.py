@@ -108,7 +108,7 @@ ROWS = dict(k=A, v=A, n=5, row=0, head=0, pages=_pages(), table=A, n_seqs=5, max
     (0, {}), (0, dict(rope=_rope())), (0, dict(rope=_rope(rot_dim=2, interleaved=1))), (0, dict(n=1000, seq=A)),
     (0, dict(row=128, head=5 * 128, written=1)), (0, dict(row=4096, head=128, written=1)), (0, dict(row=1, head=1)),
     (1, dict(k=None)), (1, dict(v=None)), (1, dict(pos=None)), (1, dict(table=None)), (1, dict(n=0)), (1, dict(n=-3)), (1, dict(n=6)),
-    (1, dict(n=2**24 + 1, seq=A)), (1, dict(n_seqs=0)), (1, dict(max_pages=0)), (1, dict(max_pages=2**27)), (1, dict(row=-1)), (1, dict(head=-1)),
+    (0, dict(n=2**23, seq=A)), (1, dict(n=2**23 + 1, seq=A)), (1, dict(n_seqs=0)), (1, dict(max_pages=0)), (1, dict(max_pages=2**27)), (1, dict(row=-1)), (1, dict(head=-1)),
     (1, dict(row=2**41)), (1, dict(rope=_rope(rot_dim=130))), (1, dict(rope=_rope(rot_dim=3))), (1, dict(rope=_rope(rot_dim=0))),
     (1, dict(rope=_rope(cos=None))), (1, dict(rope=_rope(sin=None))), (1, dict(rope=_rope(max_pos=0))), (1, dict(rope=_rope(interleaved=2))),
     # rows written over each other
