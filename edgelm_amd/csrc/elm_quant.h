@@ -51,7 +51,7 @@ ELM_HOSTDEV static inline void elm_q8_group(const float* v, float safe, int* q) 
 // quotient, and adding 1/2 rounds either by at most M 2^-24, so both sums have one floor unless one lies within M 2^-20 of a
 // whole number. Such a group, and a scale outside [2^-100, 2^100], is redone with the divisions.
 template <int N, int LO, int HI>
-ELM_HOSTDEV static inline void elm_level_group(const float* v, float s, int* q) {
+ELM_HOSTDEV static inline void elm_level_group(const float* v, float s, float* level) {
   constexpr float kNear = 0.5f - (HI > 8 ? 0x1p-13f : 0x1p-17f);
 #ifdef __HIP_DEVICE_COMPILE__
   const float r = __builtin_amdgcn_rcpf(s);
@@ -74,7 +74,14 @@ ELM_HOSTDEV static inline void elm_level_group(const float* v, float s, int* q) 
     }
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i) q[i] = (int)fminf((float)HI, fmaxf((float)LO, copysignf(f[i], t[i])));
+  for (int i = 0; i < N; ++i) {
+    const float l = copysignf(f[i], t[i]);
+#ifdef __HIP_DEVICE_COMPILE__
+    level[i] = __builtin_amdgcn_fmed3f(l, (float)LO, (float)HI);
+#else
+    level[i] = fminf((float)HI, fmaxf((float)LO, l));
+#endif
+  }
 }
 
 // Byte offset of the 16 elements h*16 .. h*16+15 of token t's block b in the block-scale GEMM's

@@ -379,27 +379,33 @@ __global__ __launch_bounds__(256) void paged_append_kernel(RowArgs a) {
     const float s = amax / 127.f, div = s == 0.f ? 1.f : s;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      int q[4];
+      float q[4];
       elm_level_group<4, -127, 127>(x[j], div, q);
-      *reinterpret_cast<uint32_t*>(dst + 32 * j + 4 * c) =
-          (q[0] & 0xFF) | (q[1] & 0xFF) << 8 | (q[2] & 0xFF) << 16 | (uint32_t)(q[3] & 0xFF) << 24;
+      // bytes q + 128, two a conversion; then each less 128 again
+      const uint32_t lo = (uint32_t)fmaf(q[1], 256.f, q[0] + 32896.f), hi = (uint32_t)fmaf(q[3], 256.f, q[2] + 32896.f);
+      *reinterpret_cast<uint32_t*>(dst + 32 * j + 4 * c) = (lo | hi << 16) ^ 0x80808080u;
     }
     if (c == 0) scales[row] = s;
   } else {
     uint32_t b[NB];  // a group's two bytes of this lane
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      // the first value of largest magnitude: of this lane's four, then of the eight lanes (a tie is the lower lane's)
-      float m = x[j][0];
+      // the first value of largest magnitude: the largest or the smallest one, and where those are level, the first of them
+      const float up = row_max8(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+      const float down = row_max8(fmaxf(fmaxf(-x[j][0], -x[j][1]), fmaxf(-x[j][2], -x[j][3])));
+      float peak = up >= down ? up : -down;
+      if (__any(up == down && up != 0.f)) {
+        float m = x[j][0];
 #pragma unroll
-      for (int e = 1; e < 4; ++e) m = fabsf(x[j][e]) > fabsf(m) ? x[j][e] : m;
-      const float amax = row_max8(fabsf(m));
-      const uint32_t have = (uint32_t)(__ballot(fabsf(m) == amax) >> (threadIdx.x & 56)) & 0xFFu;
-      // no lane has it only if a value is not a number
-      const float s = __shfl(m, (threadIdx.x & 56) + (have ? __builtin_ctz(have) : 0), 64) / -8.f, div = s == 0.f ? 1.f : s;
-      int q[4];
+        for (int e = 1; e < 4; ++e) m = fabsf(x[j][e]) > fabsf(m) ? x[j][e] : m;
+        const uint32_t have = (uint32_t)(__ballot(fabsf(m) == fmaxf(up, down)) >> (threadIdx.x & 56)) & 0xFFu;
+        peak = __shfl(m, (threadIdx.x & 56) + (have ? __builtin_ctz(have) : 0), 64);  // have: 0 only where a value is no number
+      }
+      const float s = peak / -8.f, div = s == 0.f ? 1.f : s;
+      float q[4];
       elm_level_group<4, -8, 7>(x[j], div, q);
-      b[j] = (uint32_t)(q[0] + 8) | (uint32_t)(q[1] + 8) << 4 | (uint32_t)(q[2] + 8) << 8 | (uint32_t)(q[3] + 8) << 12;
+      // four nibbles q + 8 in one conversion: whole numbers under 2^16
+      b[j] = (uint32_t)fmaf(q[3], 4096.f, fmaf(q[2], 256.f, fmaf(q[1], 16.f, q[0] + 34952.f)));
       if (c == 0) scales[kv_scale(w.page, h, w.slot, pg.n_kv, pg.page_size, NB) + (int64_t)j * pg.page_size] = s;
     }
     if (keys) {  // [c / 2][j]: words of which this lane has one half; the even lane stores them

@@ -13,10 +13,10 @@ SHIM = r"""
 #include <cmath>
 #define ELM_HOSTDEV
 #include "elm_quant.h"
-extern "C" void levels4(const float* v, const float* s, long groups, int* q) {
+extern "C" void levels4(const float* v, const float* s, long groups, float* q) {
   for (long g = 0; g < groups; ++g) elm_level_group<4, -8, 7>(v + 4 * g, s[g], q + 4 * g);
 }
-extern "C" void levels8(const float* v, const float* s, long groups, int* q) {
+extern "C" void levels8(const float* v, const float* s, long groups, float* q) {
   for (long g = 0; g < groups; ++g) elm_level_group<4, -127, 127>(v + 4 * g, s[g], q + 4 * g);
 }
 """
@@ -42,6 +42,6 @@ def test_one_reciprocal_gives_the_quotients_levels(tmp_path, bits, lo, hi):
         v[~np.isfinite(v)] = 0
         r = v / s[:, None]
         want = np.clip(np.copysign(np.floor(np.abs(r) + np.float32(0.5)), r), lo, hi).astype(np.int32)
-    got, v = np.empty((n, 4), np.int32), np.ascontiguousarray(v)
+    got, v = np.empty((n, 4), np.float32), np.ascontiguousarray(v)
     getattr(lib, f"levels{bits}")(v.ctypes.data_as(C.c_void_p), s.ctypes.data_as(C.c_void_p), C.c_long(n), got.ctypes.data_as(C.c_void_p))
     assert np.array_equal(got, want), np.argwhere(got != want)[:5]
