@@ -567,6 +567,8 @@ __device__ __forceinline__ void split8(const float* x, u32x4* out, float minus_o
 
 // Levels as f16, two an instruction. A small integer u in the low bits of a half is the subnormal u 2^-24, and the fused
 // multiply-add takes it to (u - bias) 2^-9, exactly: levels are held times 2^-9 (kLevelExp), which the final factor undoes.
+// (The subnormals themselves as operands, their bias taken off a score's sum, save the multiply-add but give errors of 2.7e-6
+// in place of 2.8e-7: the matrix instruction aligns a subnormal's product by its exponent, not by its leading bit.)
 constexpr int kLevelExp = 9;
 __device__ __forceinline__ uint32_t f16_levels(uint32_t w, float mul, float add) {
   const f16x2 r = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)mul, (_Float16)mul},
@@ -578,6 +580,8 @@ __device__ __forceinline__ uint32_t f16_bytes(uint32_t w) { return f16_levels(w,
 // nibbles q + 8 at bits 0-3, and at bits 4-7 (16 u 2^-24 times 2^11)
 __device__ __forceinline__ uint32_t f16_low_nibbles(uint32_t w) { return f16_levels(w & 0x000F000Fu, 0x1p15f, -0x1p-6f); }
 __device__ __forceinline__ uint32_t f16_high_nibbles(uint32_t w) { return f16_levels(w & 0x00F000F0u, 0x1p11f, -0x1p-6f); }
+// a whole byte of two nibbles: 16 (q1 + 8) + (q0 + 8) - 136
+__device__ __forceinline__ uint32_t f16_nibble_bytes(uint32_t w) { return f16_levels(w, 0x1p15f, -136 * 0x1p-9f); }
 
 // ---- which values of a row a lane holds. Lane = 16 g + n.
 // Keys (rows of the 16 x 32 operand are tokens, n): step j's eight values of lane group g.
@@ -724,7 +728,8 @@ __device__ __forceinline__ void load_value(const uint8_t* row, uint32_t off, int
     }
   }
 }
-// The operand of value x over eight tokens: v[0..3] the first block's, v[4..7] the second's
+// The operand of value x over eight tokens: v[0..3] the first block's, v[4..7] the second's. q4: of an odd x the byte that holds it
+// and its neighbour, 16 times the one plus the other: the neighbour's sum is taken off at the end (after the last tile).
 template <int DT, int NB>
 __device__ __forceinline__ u32x4 value_operand(const uint32_t (&v)[8][value_words(DT, NB)], int x) {
   u32x4 o;
@@ -738,7 +743,7 @@ __device__ __forceinline__ u32x4 value_operand(const uint32_t (&v)[8][value_word
       const int j = x / 2;
       const uint32_t sel = 0x0C040C00u + (j % 4) * 0x00010001u;
       const uint32_t w = __builtin_amdgcn_perm(v[2 * i + 1][j / 4], v[2 * i][j / 4], sel);
-      o[i] = x % 2 ? f16_high_nibbles(w) : f16_low_nibbles(w);
+      o[i] = x % 2 ? f16_nibble_bytes(w) : f16_low_nibbles(w);
     } else {
       o[i] = __builtin_amdgcn_perm(v[2 * i + 1][x / 2], v[2 * i][x / 2], x % 2 ? 0x07060302u : 0x05040100u);
     }
@@ -836,7 +841,7 @@ struct PagedRegs {
 // COLS (q4, where the heads times the NB groups of 32 fit in the 16 columns): column n = h + j 16 / NB is head h and group j. Its
 // query is zero outside the group, so a score's NB parts come out in NB lanes, each multiplied by its own group's scale and
 // then added over them; and its weights take its own group's value scales, so that one split of 8 weights serves in place of
-// NB (344 vector instructions a tile for 476).
+// NB.
 template <int DT, int NB, bool COLS>
 __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int HD = 32 * NB, OP = op_of(DT), PC = pieces_of(DT);
@@ -1027,7 +1032,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
         } else if constexpr (DT == ELMH_Q8) {
           v *= row_bcast<u>(r.ks[0][i]);
         }
-        s[4 * u + i] = v * scale;
+        s[4 * u + i] = v;
       }
     });
     const PagedTile now = tile;
@@ -1043,11 +1048,11 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
     }
 
     const float top = max_of(max_of(max_of(max_of(s[0], s[1]), s[2]), max_of(max_of(s[3], s[4]), s[5])), max_of(s[6], s[7]));
-    const float mn = max_of(m, max_over_groups(top));
+    const float mn = max_of(m, max_over_groups(top) * scale);
     const float ref = mn == -INFINITY ? 0.f : mn;  // no token so far: weights of 0, not of exp(-inf + inf)
     float p[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], scale, -ref));
     float fade = __builtin_amdgcn_exp2f(m - ref);
     m = mn;
     l = l * fade + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
@@ -1133,6 +1138,12 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
+  if constexpr (DT == ELMH_Q4) {  // value_operand
+#pragma unroll
+    for (int x = 1; x < 2 * NB; x += 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[x][i] = (acc[x][i] - acc[x - 1][i]) * 0x1p-4f;
+  }
   // the waves' sums joined: o = sum_w 2^(m_w - M) o_w
   if constexpr (OP == kOpF16) {
     const float f = pow2((NG ? vexp + kLevelExp : 0) - 14);

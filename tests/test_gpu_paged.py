@@ -351,6 +351,31 @@ def test_attention_of_uneven_scales(ctx, dtype):
     c.free()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("grp", [4, 8])
+def test_attention_is_as_exact_as_f32(ctx, dtype, grp):
+    """Queries, weights and sums keep their 24 bits. Scores of unit variance over 128 products: the partial sums of an f32
+    accumulation grow to the score's size, each rounded by up to half a step, a third of that on average of squares:
+    sqrt(128 / 3) = 6.5 half steps of error, which the weights carry into the output; rounding the queries, the scores, the weights and
+    the output adds some two. 16 half steps leave a factor of two; pieces of one 16-bit type less would be a hundred off."""
+    rng = np.random.default_rng(23)
+    page, n_kv, hd, n_pages, lens = 16, 2, 128, 64, [1024, 1000]
+    table = np.stack([rng.permutation(n_pages) for _ in lens]).astype(np.int32)
+    c = Cache(ctx, dtype, n_kv, hd, page, n_pages)
+    for p in range(n_pages):
+        for h in range(n_kv):
+            for s in range(page):
+                c.put("k", p, h, s, rng.normal(0, 1, hd))
+                c.put("v", p, h, s, rng.normal(0, 1, hd))
+    c.send()
+    q = rng.normal(0, 1, (2, n_kv * grp, hd)).astype(np.float32)
+    want, _ = _attention64(c, q, table, lens)
+    got = _attend(ctx, c, q, table, lens)
+    rel = np.linalg.norm(got - want) / np.linalg.norm(want)
+    assert rel <= 16 * EPS, rel / EPS
+    c.free()
+
+
 @pytest.mark.parametrize("dtype", ["q8", "q4", "f32", "bf16"])
 @pytest.mark.parametrize("k_amp,v_amp,q_amp", [(1e-30, 1e34, 1e30), (1e30, 1e-34, 1e-30)])
 def test_attention_at_the_ends_of_the_range(ctx, dtype, k_amp, v_amp, q_amp):
@@ -790,6 +815,34 @@ def test_decode_step_in_graphs(ctx):
     _free(tb, kb, vb, sb, pb, q, kn, vn, pos, lens, o, o2)
     c.free()
     r.free()
+
+
+def test_two_contexts_at_once(ctx):
+    """Calls on two contexts' streams in flight together, each with split sequences and its own scratch."""
+    rng = np.random.default_rng(41)
+    other = E.Context(0)
+    sides = []
+    for c in (ctx, other):
+        cache = Cache(c, "bf16", 2, 64, 16, 30)
+        lens = [3000, 17, 2100]
+        table = rng.integers(0, 30, (3, 190)).astype(np.int32)
+        for p in range(30):
+            for h in range(2):
+                for s in range(16):
+                    cache.put("k", p, h, s, rng.normal(0, 1, 64))
+                    cache.put("v", p, h, s, rng.normal(0, 1, 64))
+        cache.send()
+        q = rng.normal(0, 1, (3, 8, 64)).astype(np.float32)
+        sides.append((c, cache, q, _up(c, q, table, np.array(lens, np.int32), q), _attend(c, cache, q, table, lens)))
+    for _ in range(20):
+        for c, cache, q, (qb, tb, lb, ob), _ in sides:
+            for _ in range(5):
+                c.paged_attention_dev(qb.ptr, ob.ptr, 8, cache.pages, tb.ptr, 3, 190, lb.ptr, 3000)
+    for c, cache, q, bufs, want in sides:
+        assert np.array_equal(bufs[3].download(q.shape, np.float32), want)
+        _free(*bufs)
+        cache.free()
+    other.close()
 
 
 def test_scratch_does_not_grow_in_a_capture():
