@@ -234,6 +234,24 @@ def test_attention_groups(ctx, dtype, grp):
     c.free()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,grp", [(256, 16), (256, 33), (192, 16), (128, 32)])
+def test_attention_of_wide_tiles(ctx, dtype, hd, grp):
+    """All sixteen columns at the large head sizes (66 KB of LDS at 256), split and in one part."""
+    rng = np.random.default_rng([hd, grp])
+    lens, page, n_kv = [600, 0, 40], 64, 1
+    table = _table_of(rng, lens, page, 12)
+    c = Cache(ctx, dtype, n_kv, hd, page, 12)
+    _fill(c, rng, table, lens)
+    c.send()
+    q = rng.normal(0, 1, (3, grp, hd)).astype(np.float32)
+    want, tol = _attention64(c, q, table, lens)
+    _check(_attend(ctx, c, q, table, lens), want, tol)
+    want, tol = _attention64(c, q, table, [512, 0, 40])
+    _check(_attend(ctx, c, q, table, lens, max_len=512), want, tol)
+    c.free()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "q8"])
 @pytest.mark.parametrize("rot,inter", [(128, False), (128, True), (64, False), (20, True), (22, False), (2, False)])
 def test_attention_rotates_queries(ctx, dtype, rot, inter):
