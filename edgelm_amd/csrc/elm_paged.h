@@ -63,8 +63,6 @@ ELM_HD int64_t kv_page_of(const int32_t* table_row, int max_pages, int64_t n_pag
 
 // ---------------------------------------------------------------- the split of a sequence
 
-ELM_HD int split_parts(int units, int per) { return (units + per - 1) / per; }
-
 constexpr int kPartLeastUnits = 4;   // of a part: one unit a wave
 constexpr int kPartAloneUnits = 16;  // sequences up to this are not split: the second launch costs more (q8, 200 positions: 8.5 us
                                      // in one, 11.6 split; 500: 10.7 and 11.5; 1000: 14.4 and 11.5)
@@ -95,16 +93,59 @@ inline int part_few(int rows, int extra) {
   const int few = 256 / rows;
   return few < 1 ? 1 : few < extra ? few : extra;
 }
+// ceil(n / d) by a multiplication: at least that, and over it by one at most (exact while n stays under 2^32 / d)
+struct CeilDiv {
+  uint32_t below = 0;       // d - 1
+  uint32_t lo = 1, hi = 1;  // floor(2^32 / d) + 1
+};
+inline CeilDiv ceil_div(int d) {
+  const uint64_t m = (uint64_t(1) << 32) / (uint32_t)d + 1;
+  return {(uint32_t)d - 1, (uint32_t)m, (uint32_t)(m >> 32)};
+}
+ELM_HD uint32_t mul_high(uint32_t a, uint32_t b) { return (uint32_t)(((uint64_t)a * b) >> 32); }
+ELM_HD int ceil_of(int n, const CeilDiv& d) {
+  const uint32_t x = (uint32_t)n + d.below;
+  return (int)(mul_high(x, d.lo) + (d.hi ? x : 0));
+}
+
+// The rule that every workgroup applies to the batch's lengths
+struct PartRule {
+  CeilDiv few, once, extra;
+  int least = 1;
+};
+inline PartRule part_rule(int workgroups, int rows, int n_seqs, int max_len, int extra) {
+  return {ceil_div(part_few(rows, extra)), ceil_div(part_once(workgroups, rows, n_seqs, extra)), ceil_div(extra), part_least(max_len)};
+}
 // Units a part: the batch's `total` over `once`, but of kPartFairUnits as long as `few` parts (one workgroup a CU) are left; where
 // that gives parts of kPartLongUnits and more, over up to `extra`, so that uneven ends even out. (64 q4 sequences of 8 to 16
 // thousand positions, 8 kv heads: 512 workgroups 212 us, 1536 201; one bf16 sequence of 100k: 512 78 us, 1536 85.)
-ELM_HD int part_size(int total, int few, int once, int extra, int at_least) {
-  const int small = split_parts(total, once), fair = split_parts(total, few), least = split_parts(total, extra);
+ELM_HD int part_size(int total, const PartRule& r) {
+  const int small = ceil_of(total, r.once), fair = ceil_of(total, r.few), least = ceil_of(total, r.extra);
   int per = fair < kPartFairUnits ? fair : kPartFairUnits;
   if (small > per) per = small;
   if (per > kPartLongUnits) per = kPartLongUnits;
   if (least > per) per = least;
-  return per > at_least ? per : at_least;
+  return per > r.least ? per : r.least;
+}
+// Parts of a sequence (one if it is empty), and where they begin: no divisions. The quotient is taken a 2^-20th low, so that a
+// multiple of `per` units is not cut once more; a part of a very long sequence may then be longer than `per` by as much.
+ELM_HD float part_inverse(int per) {
+#ifdef __HIP_DEVICE_COMPILE__
+  return __builtin_amdgcn_rcpf((float)per) * (1.f - 0x1p-20f);
+#else
+  return 1.f / (float)per * (1.f - 0x1p-20f);
+#endif
+}
+ELM_HD int part_count(int units, float inverse) { return (int)((float)units * inverse) + 1; }
+ELM_HD int part_begin(int units, int part, int parts) {  // of part `parts`: the end
+  if (part == parts) return units;
+#ifdef __HIP_DEVICE_COMPILE__
+  const float each = (float)units * __builtin_amdgcn_rcpf((float)parts);
+#else
+  const float each = (float)units / (float)parts;
+#endif
+  const int at = (int)((float)part * each);
+  return at < units ? at : units;
 }
 
 // ---------------------------------------------------------------- what a call has to satisfy

@@ -222,10 +222,11 @@ hipError_t launch_paged_append(const float* k, const float* v, int n, int64_t ro
 hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t head, const elmh_kv_pages& pages,
                              const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq,
                              hipStream_t s);
-// How the attention splits a batch (part_few, part_once, part_extra, part_least), and the bytes of the parts' results (0 where no
+// How the attention splits a batch (part_rule, part_extra), and the bytes of the parts' results (0 where no
 // sequence of max_len is split)
 struct PagedSplit {
-  int few = 1, once = 1, extra = 1, least = 1;
+  int extra = 1;
+  PartRule rule;
   size_t part_bytes = 0;
 };
 PagedSplit paged_attention_split(int dtype, int n_seqs, int n_heads, int n_kv, int head_dim, int max_len);

@@ -764,7 +764,8 @@ struct PagedAttnArgs {
   int max_len;
   const float *cs, *sn;
   int rot, inter;
-  int n_seqs, few, once, extra, least;  // the split: PagedShare, part_size
+  int n_seqs;
+  PartRule rule;      // the split: PagedShare
   float* part_o;      // [slot][head][head_dim], unnormalized
   float* part_s;      // [slot][head][2]: running maximum (base 2), sum
   int2* joins;        // [seq]: first slot, parts; null where no sequence is split
@@ -788,17 +789,19 @@ struct PagedShare {
   int seq, len, units;
   int part, parts, first;  // which of the sequence's, of how many, the first one's slot
 };
-// The share of a slot. Uniform (every lane of the wave calls); seq < 0: the slot is no sequence's.
+// The share of a slot. Uniform (every lane of the wave calls); seq < 0: the slot is no sequence's. A workgroup's first hundreds of
+// instructions come from memory (some 10 clocks each), so there is no division among them.
 __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, int slot) {
   const int lane = threadIdx.x & 63;
   const auto len_of = [&](int i) { return i < a.n_seqs ? min(max(a.lens[i], 0), a.max_len) : 0; };
-  const auto units_of = [&](int len) { return (len + kSplitUnit - 1) / kSplitUnit; };
-  int total = 0;
-  for (int i = 0; i < a.n_seqs; i += 64) total += wave_sum_i(units_of(len_of(i + lane)));
-  const int per = part_size(total, a.few, a.once, a.extra, a.least);
-  int before = 0;
-  for (int i = 0; i < a.n_seqs; i += 64) {
-    const int len = len_of(i + lane), units = units_of(len), parts = i + lane < a.n_seqs ? max(1, split_parts(units, per)) : 0;
+  const auto units_of = [&](int len) { return (int)(((uint32_t)len + kSplitUnit - 1) / kSplitUnit); };
+  const int len0 = len_of(lane);
+  int total = wave_sum_i(units_of(len0));
+  for (int i = 64; i < a.n_seqs; i += 64) total += wave_sum_i(units_of(len_of(i + lane)));
+  const float inverse = part_inverse(part_size(total, a.rule));
+  int before = 0, i = 0, len = len0;
+  while (true) {
+    const int units = units_of(len), parts = i + lane < a.n_seqs ? part_count(units, inverse) : 0;
     const int sum = wave_scan_i(parts);
     const uint64_t past = __ballot(before + sum > slot);
     if (past) {
@@ -812,9 +815,11 @@ __device__ __forceinline__ PagedShare paged_share(const PagedAttnArgs& a, int sl
       s.part = slot - s.first;
       return s;
     }
+    i += 64;
+    if (i >= a.n_seqs) return {-1, 0, 0, 0, 0, 0};
     before += __builtin_amdgcn_readlane(sum, 63);
+    len = len_of(i + lane);
   }
-  return {-1, 0, 0, 0, 0, 0};
 }
 
 // Two blocks of 16 tokens (a wave's step): where they lie, and how many tokens of each count (0: behind the end, or no page)
@@ -848,8 +853,8 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   extern __shared__ float lds[];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.x / a.head_tiles;
-  const int h0 = kvh * a.group + blockIdx.x % a.head_tiles * kPaHeads;
+  const int kvh = blockIdx.x;
+  const int h0 = kvh * a.group + blockIdx.z * kPaHeads;
   const int heads = min(kPaHeads, (kvh + 1) * a.group - h0);
   const elmh_kv_pages& pg = a.pages;
   const PagedShare share = paged_share(a, blockIdx.y);
@@ -858,7 +863,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   float* out = a.out + (int64_t)seq * a.n_heads * HD + (int64_t)h0 * HD;
   // for the join (written last: a store ahead of the table's loads would keep them off the scalar cache)
   const auto note = [&] {
-    if (share.part == 0 && blockIdx.x == 0 && tid == 0 && a.joins) a.joins[seq] = make_int2(share.first, share.parts);
+    if (share.part == 0 && blockIdx.x + blockIdx.z == 0 && tid == 0 && a.joins) a.joins[seq] = make_int2(share.first, share.parts);
   };
   if (len == 0) {
     for (int i = tid; i < heads * HD; i += 64 * kPaWaves) out[i] = 0.f;
@@ -867,7 +872,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
   }
 
   const int32_t* trow = a.table + (int64_t)seq * a.max_pages;
-  const int ps = pg.page_size, last = (len - 1) / kPageStep;
+  const int ps = pg.page_size, last = (int)((uint32_t)(len - 1) / kPageStep);
   constexpr int RB = DT == ELMH_F32 ? 4 * HD : DT == ELMH_Q8 ? HD : DT == ELMH_Q4 ? HD / 2 : 2 * HD;
   constexpr int NG = DT == ELMH_Q8 ? 1 : DT == ELMH_Q4 ? NB : 0;
   const uint8_t* kpool = static_cast<const uint8_t*>(pg.k);
@@ -884,7 +889,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
 #pragma unroll
     for (int u = 0; u < 2; ++u) id[u] = trow[page_index(min(2 * unit + u, last) * kPageStep, a.magic)];
   };
-  const int steps = ps / kPageStep;
+  const int steps = (int)((uint32_t)ps / kPageStep);
   const auto place = [&](int unit, const int (&id)[2]) {
     PagedTile t;
 #pragma unroll
@@ -923,9 +928,8 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
     load_scales(r.vs, pg.v_scale, t);
   };
 
-  // at most 2^23 units times kPartMostExtra + 1 parts
-  const int end = (int)((uint32_t)share.units * (uint32_t)(share.part + 1) / (uint32_t)share.parts);
-  int unit = (int)((uint32_t)share.units * (uint32_t)share.part / (uint32_t)share.parts) + wave;
+  const int end = __builtin_amdgcn_readfirstlane(part_begin(share.units, share.part + 1, share.parts));
+  int unit = __builtin_amdgcn_readfirstlane(part_begin(share.units, share.part, share.parts)) + wave;
   const bool busy = unit < end;  // a wave without a unit joins with nothing
   int id[2];
   PagedTile tile;
@@ -957,35 +961,40 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
 #pragma unroll
       for (int i = 0; i < 4; ++i) qf[4 * j + i] = qrow[16 * j + 4 * g + i];
   } else {
-    float up = 1.f;
+    constexpr int QJ = COLS ? 1 : NB;  // groups that a lane reads: with COLS its own
+    float x[QJ][8];
+#pragma unroll
+    for (int j = 0; j < QJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[j][e] = qrow[32 * sj * COLS + key_dim<DT, NB>(j, g, e)];
     if constexpr (OP == kOpF16) {  // the head's largest value to 512 .. 1024: its 24 bits then lie in f16's range
       float big = 0.f;
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
+      for (int j = 0; j < QJ; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(qrow[32 * j + 8 * g + e]));
-      big = max_over_groups(big);  // (with COLS every lane of a head reads all of its groups)
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[j][e]));
+      big = max_over_groups(big);
+      if constexpr (COLS) {
+        big = max_of(big, dpp_f<kDppRowRor8>(big));
+        if constexpr (NB >= 4) big = max_of(big, dpp_f<kDppRowRor4>(big));
+        if constexpr (NB >= 8) big = max_of(big, dpp_f<kDppRowRor2>(big));
+      }
       const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 127);
-      up = pow2(9 - ex);
+      const float up = pow2(9 - ex);
       scale *= pow2(ex - 9 + (NG ? kLevelExp : 0));
+#pragma unroll
+      for (int j = 0; j < QJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[j][e] *= up;
     }
+#pragma unroll
+    for (int j = 0; j < QJ; ++j) split8<OP>(x[j], qo[j], minus_one);
     if constexpr (COLS) {
-      float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = qrow[32 * sj + key_dim<DT, NB>(0, g, e)] * up;
-      u32x4 o[PC];
-      split8<OP>(x, o, minus_one);
+      for (int p = 0; p < PC; ++p) {
+        const u32x4 o = qo[0][p];
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int p = 0; p < PC; ++p) qo[j][p] = sj == j ? o[p] : u32x4{0, 0, 0, 0};
-    } else {
-#pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = qrow[key_dim<DT, NB>(j, g, e)] * up;
-        split8<OP>(x, qo[j], minus_one);
+        for (int j = 0; j < NB; ++j) qo[j][p] = sj == j ? o : u32x4{0, 0, 0, 0};
       }
     }
   }
@@ -1145,13 +1154,6 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
       for (int i = 0; i < 4; ++i) acc[x][i] = (acc[x][i] - acc[x - 1][i]) * 0x1p-4f;
   }
   // the waves' sums joined: o = sum_w 2^(m_w - M) o_w
-  if constexpr (OP == kOpF16) {
-    const float f = pow2((NG ? vexp + kLevelExp : 0) - 14);
-#pragma unroll
-    for (int x = 0; x < 2 * NB; ++x)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[x][i] *= f;
-  }
   lds_barrier();  // the queries have been read
   float* stat = lds + kPaWaves * heads * HD;
   if (qn < heads) {
@@ -1164,6 +1166,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
     if (g == 0 && qn == n) {
       stat[wave * kPaHeads + n] = m;
       stat[(kPaWaves + wave) * kPaHeads + n] = l;
+      if (n == 0) stat[2 * kPaWaves * kPaHeads + wave] = OP == kOpF16 ? pow2((NG ? vexp + kLevelExp : 0) - 14) : 1.f;
     }
   }
   lds_barrier();
@@ -1177,7 +1180,7 @@ __global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attentio
 #pragma unroll
     for (int w = 0; w < kPaWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(stat[w * kPaHeads + h] - ref);
-      o += f * lds[(w * heads + h) * HD + d];
+      o += f * stat[2 * kPaWaves * kPaHeads + w] * lds[(w * heads + h) * HD + d];
       L += f * stat[(kPaWaves + w) * kPaHeads + h];
     }
     if (share.parts == 1) {
@@ -1263,14 +1266,14 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs 
 }
 
 template <int DT, int NB, bool COLS>
-hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, hipStream_t s) {
+hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, int extra, hipStream_t s) {
   const int heads = a.group < kPaHeads ? a.group : kPaHeads;
-  const size_t lds = (size_t)(kPaWaves * heads * 32 * NB + 2 * kPaWaves * kPaHeads) * sizeof(float);
+  const size_t lds = (size_t)(kPaWaves * heads * 32 * NB + 2 * kPaWaves * kPaHeads + kPaWaves) * sizeof(float);
   if (lds > 64 * 1024) {
     static DeviceOnce once;
     if (!raise_dynamic_lds(once, (const void*)paged_attention_kernel<DT, NB, COLS>, 80 * 1024)) return hipErrorInvalidValue;
   }
-  const dim3 grid(a.pages.n_kv * a.head_tiles, n_seqs + a.extra);  // slots of no sequence come last
+  const dim3 grid(a.pages.n_kv, n_seqs + extra, a.head_tiles);  // slots of no sequence come last
   paged_attention_kernel<DT, NB, COLS><<<grid, 64 * kPaWaves, lds, s>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.part_o) return e;
@@ -1278,20 +1281,20 @@ hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, hipStre
   return hipGetLastError();
 }
 template <int DT, int NB>
-hipError_t launch_paged_attention_cols(const PagedAttnArgs& a, int n_seqs, hipStream_t s) {
+hipError_t launch_paged_attention_cols(const PagedAttnArgs& a, int n_seqs, int extra, hipStream_t s) {
   if constexpr (DT == ELMH_Q4 && (NB == 2 || NB == 4 || NB == 8))
-    if (a.group * NB <= kPaHeads) return launch_paged_attention_as<DT, NB, true>(a, n_seqs, s);
-  return launch_paged_attention_as<DT, NB, false>(a, n_seqs, s);
+    if (a.group * NB <= kPaHeads) return launch_paged_attention_as<DT, NB, true>(a, n_seqs, extra, s);
+  return launch_paged_attention_as<DT, NB, false>(a, n_seqs, extra, s);
 }
 template <int DT>
-hipError_t launch_paged_attention_of(const PagedAttnArgs& a, int n_seqs, hipStream_t s) {
+hipError_t launch_paged_attention_of(const PagedAttnArgs& a, int n_seqs, int extra, hipStream_t s) {
   switch (a.pages.head_dim) {
-    case 32: return launch_paged_attention_cols<DT, 1>(a, n_seqs, s);
-    case 64: return launch_paged_attention_cols<DT, 2>(a, n_seqs, s);
-    case 96: return launch_paged_attention_cols<DT, 3>(a, n_seqs, s);
-    case 128: return launch_paged_attention_cols<DT, 4>(a, n_seqs, s);
-    case 192: return launch_paged_attention_cols<DT, 6>(a, n_seqs, s);
-    case 256: return launch_paged_attention_cols<DT, 8>(a, n_seqs, s);
+    case 32: return launch_paged_attention_cols<DT, 1>(a, n_seqs, extra, s);
+    case 64: return launch_paged_attention_cols<DT, 2>(a, n_seqs, extra, s);
+    case 96: return launch_paged_attention_cols<DT, 3>(a, n_seqs, extra, s);
+    case 128: return launch_paged_attention_cols<DT, 4>(a, n_seqs, extra, s);
+    case 192: return launch_paged_attention_cols<DT, 6>(a, n_seqs, extra, s);
+    case 256: return launch_paged_attention_cols<DT, 8>(a, n_seqs, extra, s);
   }
   return hipErrorInvalidValue;
 }
@@ -1421,12 +1424,11 @@ hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t hea
 
 PagedSplit paged_attention_split(int dtype, int n_seqs, int n_heads, int n_kv, int head_dim, int max_len) {
   const int rows = n_kv * ((n_heads / n_kv + kPaHeads - 1) / kPaHeads);
+  const int workgroups = part_workgroups(dtype, head_dim);
   PagedSplit p;
-  p.extra = part_extra(part_workgroups(dtype, head_dim), rows, n_seqs, max_len);
-  p.once = part_once(part_workgroups(dtype, head_dim), rows, n_seqs, p.extra);
-  p.few = part_few(rows, p.extra);
-  p.least = part_least(max_len);
-  if (max_len > p.least * kSplitUnit)
+  p.extra = part_extra(workgroups, rows, n_seqs, max_len);
+  p.rule = part_rule(workgroups, rows, n_seqs, max_len, p.extra);
+  if (max_len > p.rule.least * kSplitUnit)
     p.part_bytes = ((size_t)n_seqs + p.extra) * n_heads * (head_dim + 2) * sizeof(float) + n_seqs * sizeof(int2);
   return p;
 }
@@ -1454,21 +1456,18 @@ hipError_t launch_paged_attention(const float* q, float* out, int64_t q_row, int
   }
   a.magic = page_magic(pages.page_size);
   a.n_seqs = n_seqs;
-  a.few = split.few;
-  a.least = split.least;
-  a.once = split.once;
-  a.extra = split.extra;
+  a.rule = split.rule;
   if (split.part_bytes) {
     a.part_o = parts;
     a.part_s = parts + ((int64_t)n_seqs + split.extra) * n_heads * pages.head_dim;
     a.joins = reinterpret_cast<int2*>(a.part_s + ((int64_t)n_seqs + split.extra) * n_heads * 2);
   }
   switch (pages.dtype) {
-    case ELMH_F32: return launch_paged_attention_of<ELMH_F32>(a, n_seqs, s);
-    case ELMH_F16: return launch_paged_attention_of<ELMH_F16>(a, n_seqs, s);
-    case ELMH_BF16: return launch_paged_attention_of<ELMH_BF16>(a, n_seqs, s);
-    case ELMH_Q8: return launch_paged_attention_of<ELMH_Q8>(a, n_seqs, s);
-    case ELMH_Q4: return launch_paged_attention_of<ELMH_Q4>(a, n_seqs, s);
+    case ELMH_F32: return launch_paged_attention_of<ELMH_F32>(a, n_seqs, split.extra, s);
+    case ELMH_F16: return launch_paged_attention_of<ELMH_F16>(a, n_seqs, split.extra, s);
+    case ELMH_BF16: return launch_paged_attention_of<ELMH_BF16>(a, n_seqs, split.extra, s);
+    case ELMH_Q8: return launch_paged_attention_of<ELMH_Q8>(a, n_seqs, split.extra, s);
+    case ELMH_Q4: return launch_paged_attention_of<ELMH_Q4>(a, n_seqs, split.extra, s);
   }
   return hipErrorInvalidValue;
 }

@@ -35,12 +35,13 @@ int table(const float* c, const float* s, int64_t p0, int64_t n, int rot, double
 }
 int64_t page_of(const int32_t* row, int mp, int64_t np, int pos, int ps) { return kv_page_of(row, mp, np, pos, page_magic(ps)); }
 int page_index_of(int pos, int ps) { return page_index(pos, page_magic(ps)); }
-int parts_of(int units, int per) { return split_parts(units, per); }
 int extra(int dt, int hd, int rows, int n, int max_len) { return part_extra(part_workgroups(dt, hd), rows, n, max_len); }
-int once(int dt, int hd, int rows, int n, int extra) { return part_once(part_workgroups(dt, hd), rows, n, extra); }
-int few(int rows, int extra) { return part_few(rows, extra); }
-int least(int max_len) { return part_least(max_len); }
-int size(int total, int few, int once, int extra, int least) { return part_size(total, few, once, extra, least); }
+int size(int dt, int hd, int rows, int n, int max_len, int extra, int total) {
+  return part_size(total, part_rule(part_workgroups(dt, hd), rows, n, max_len, extra));
+}
+int count(int units, int per) { return part_count(units, part_inverse(per)); }
+int begin(int units, int part, int parts) { return part_begin(units, part, parts); }
+int ceil_div_of(int n, int d) { return ceil_of(n, ceil_div(d)); }
 int kbyte(int d, int hd) { return q4_key_byte(d, hd); }
 int vbyte(int d, int hd) { return q4_value_byte(d, hd); }
 double freq(int rot, double th, const elmh_rope_scaling* sc, int i) {
@@ -188,25 +189,49 @@ def test_page_index_is_the_quotient(host):
             assert host.page_index_of(pos, ps) == pos // ps, (pos, ps)
 
 
+def test_ceil_of_a_quotient(host):
+    rng = np.random.default_rng(1)
+    for d in list(range(1, 1025, 31)) + [2, 3, 64, 512, 1024]:
+        for n in [0, 1, d - 1, d, d + 1, 5 * d, 5 * d + 1, 2**30, 2**30 - 1] + rng.integers(0, 2**30, 20).tolist():
+            got, want = host.ceil_div_of(n, d), -(-n // d)
+            assert want <= got <= want + (n + d >= 2**32 // d), (n, d)
+
+
 def test_parts_fit_their_slots(host):
     """Whatever the lengths below the host's bound, the parts of all sequences (one of an empty one) are no more than n_seqs +
-    extra, each is of kPartLeastUnits or more unless its sequence is shorter, and a part's bounds are 32-bit products."""
+    extra, and a batch of short sequences is not split."""
     rng = np.random.default_rng(0)
     for rows, hd, dt in ((1, 64, E.F32), (3, 64, E.Q8), (8, 128, E.BF16), (8, 128, E.Q4), (8, 256, E.F16), (40, 128, E.Q8), (1024, 128, E.F32), (16384, 32, E.Q4)):
         for n in (1, 2, 7, 64, 65, 300, 4096):
-            for max_len in (1, 31, 128, 129, 4096, 100003, 2**23):
+            for max_len in (1, 31, 128, 512, 513, 4096, 100003, 2**23, 2**28):
+                if n * max_len > 2**35:
+                    continue
                 extra = host.extra(dt, hd, rows, n, max_len)
-                once = host.once(dt, hd, rows, n, extra)
-                assert 1 <= once <= extra <= 1024
+                assert 1 <= extra <= 1024
                 top = -(-max_len // 32)
                 for units in (np.full(n, top), rng.integers(0, top + 1, n), np.where(np.arange(n) == n // 2, top, 0), np.zeros(n, int),
                               np.where(rng.random(n) < 0.5, top, 1)):
-                    per = host.size(int(units.sum()), host.few(rows, extra), once, extra, host.least(max_len))
-                    parts = np.maximum(1, -(-units // per))
-                    assert per >= 4 and parts.sum() <= n + extra, (rows, n, max_len)
-                    assert max_len > 512 or parts.max() == 1
-                    assert parts.max() <= extra + 1 and int(units.max()) * (int(parts.max()) + 1) < 2**32
-                    assert host.parts_of(int(units[0]), per) == -(-int(units[0]) // per)
+                    per = host.size(dt, hd, rows, n, max_len, extra, int(units.sum()))
+                    parts = [host.count(int(u), per) for u in units]
+                    assert per >= 4 and min(parts) >= 1 and sum(parts) <= n + extra, (rows, n, max_len)
+                    assert max(parts) <= extra + 1
+                    assert max_len > 512 or max(parts) == 1
+
+
+def test_parts_cover_a_sequence(host):
+    """From the first unit to the last, in order, none empty while there are as many units as parts."""
+    for units in (1, 2, 4, 5, 13, 100, 999, 4097, 2**18, 2**23 - 1, 2**23):
+        for per in (4, 5, 12, 16, 33, 64, 1000, 8192, 2**23):
+            parts = host.count(units, per)
+            # the quotient is taken 2^-20 low, give or take two roundings of 2^-24; one is added to its floor
+            assert parts == -(-units // per) or (units > 2**19 and abs(parts - units / per) <= 1 + units / per * 2.0**-19), (units, per)
+            if parts > 1100:
+                continue
+            at = [host.begin(units, p, parts) for p in range(parts + 1)]
+            assert at[0] == 0 and at[-1] == units
+            assert all(b > a for a, b in zip(at, at[1:]))
+            assert max(b - a for a, b in zip(at, at[1:])) <= max(per, units / parts) + 2
+    assert host.count(0, 4) == 1
 
 
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 192, 256])
