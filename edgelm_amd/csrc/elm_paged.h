@@ -224,6 +224,7 @@ inline PagedFault check_paged_rows(const float* k, const float* v, int64_t n, in
                                    const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages,
                                    const int32_t* pos, const int32_t* seq, const elmh_rope* rope, bool written) {
   if (!k || !v) return {ELMH_ERR_ARG, "null keys or values"};
+  if (written && k == v) return {ELMH_ERR_ARG, "keys and values overlap"};
   PagedFault f = check_kv_pages(pages);
   if (!f.code) f = check_table(table, n_seqs, max_pages, pages->page_size);
   if (!f.code) f = check_rows(n, row, head, pages->n_kv, pages->head_dim, written);

@@ -306,8 +306,8 @@ int elmh_paged_append_dev(elmh_ctx* ctx, const float* k, const float* v, int n, 
                           const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages, const int32_t* pos,
                           const int32_t* seq, const elmh_rope* rope);
 /* The reverse: the values that the cache holds (level * scale, in f32) of n positions, keys as stored (rotated). Skipped rows
- * are left as they were. With row = head_dim and head = n * head_dim the rows form a contiguous cache
- * [n_kv][n][head_dim] as elmh_attention_dev keeps it. */
+ * are left as they were; no two rows written, and not k and v, may share a value. With row = head_dim and head = n *
+ * head_dim the rows form a contiguous cache [n_kv][n][head_dim] as elmh_attention_dev keeps it. */
 int elmh_paged_read_dev(elmh_ctx* ctx, float* k, float* v, int n, int64_t row, int64_t head, const elmh_kv_pages* pages,
                         const int32_t* table, int n_seqs, int max_pages, const int32_t* pos, const int32_t* seq);
 /* Attention of one new token a sequence: out[s, h] = softmax over positions p < lens[s] of (q . k_p) / sqrt(head_dim), applied

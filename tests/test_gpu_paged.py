@@ -423,7 +423,7 @@ def test_attention_of_many_sequences(ctx, dtype, hd):
             c.put("v", p, 0, s, rng.normal(0, 1, hd))
     c.send()
     rows = {(n, p): np.stack([c.get(n, p, 0, s) for s in range(page)]) for n in "kv" for p in range(n_pages)}
-    for n in (64, 65, 300):
+    for n in (64, 65, 300) + ((4096,) if dtype == "q8" else ()):
         lens = rng.integers(0, 60, n)
         lens[rng.random(n) < 0.3] = 0
         lens[[0, n // 2, n - 1]] = [3000, 1700, 2500]

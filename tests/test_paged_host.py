@@ -102,12 +102,13 @@ def test_null_pages(host):
     assert host.pages(None) == 1
 
 
-ROWS = dict(k=A, v=A, n=5, row=0, head=0, pages=_pages(), table=A, n_seqs=5, max_pages=10, pos=A, seq=None, rope=None, written=0)
+ROWS = dict(k=A, v=2 * A, n=5, row=0, head=0, pages=_pages(), table=A, n_seqs=5, max_pages=10, pos=A, seq=None, rope=None, written=0)
 
 
 @pytest.mark.parametrize("code,kw", [
     (0, {}), (0, dict(rope=_rope())), (0, dict(rope=_rope(rot_dim=2, interleaved=1))), (0, dict(n=1000, seq=A)),
     (0, dict(row=128, head=5 * 128, written=1)), (0, dict(row=4096, head=128, written=1)), (0, dict(row=1, head=1)),
+    (0, dict(k=2 * A)), (1, dict(k=2 * A, written=1)),
     (1, dict(k=None)), (1, dict(v=None)), (1, dict(pos=None)), (1, dict(table=None)), (1, dict(n=0)), (1, dict(n=-3)), (1, dict(n=6)),
     (0, dict(n=2**23, seq=A)), (1, dict(n=2**23 + 1, seq=A)), (1, dict(n_seqs=0)), (1, dict(max_pages=0)), (1, dict(max_pages=2**27)), (1, dict(row=-1)), (1, dict(head=-1)),
     (1, dict(row=2**41)), (1, dict(rope=_rope(rot_dim=130))), (1, dict(rope=_rope(rot_dim=3))), (1, dict(rope=_rope(rot_dim=0))),
