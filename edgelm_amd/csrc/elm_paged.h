@@ -70,9 +70,15 @@ inline int part_least(int max_len) { return max_len <= kPartAloneUnits * kSplitU
 constexpr int kPartFairUnits = 12;   // a part that is worth its start and end
 constexpr int kPartLongUnits = 64;   // a part whose start and end no longer matter
 constexpr int kPartMostExtra = 1024;
-// Workgroups that are on the card together: as many a CU as the kernel's registers leave room for, one to four
-inline int part_workgroups(int dtype, int head_dim) {
-  return 256 * (head_dim > 128 ? 1 : head_dim <= 64 ? 4 : dtype == ELMH_F32 || dtype == ELMH_BF16 ? 2 : 3);
+// Workgroups that are on the card together: as many a CU as the kernel's registers leave room for, one to four. Above a head size
+// of 128 two fit where the cache has few bytes (256 registers a lane without spilling: a 16-bit type to 192, q8, q4 to 192), and
+// are worth up to a sixth (8 sequences of 4 to 8 thousand, 4 kv heads: q4 of 192 24.2 us, with one 28.8; q8 of 256 36 and 37).
+constexpr bool part_two_wide(int dtype, int head_dim) {
+  return dtype == ELMH_Q8 || (dtype != ELMH_F32 && head_dim <= 192);
+}
+constexpr int part_workgroups(int dtype, int head_dim) {
+  if (head_dim > 128) return 256 * (part_two_wide(dtype, head_dim) ? 2 : 1);
+  return 256 * (head_dim <= 64 ? 4 : dtype == ELMH_F32 || dtype == ELMH_BF16 ? 2 : 3);
 }
 // Parts beside one a sequence: three times the workgroups on the card, over the `rows` (kv heads times their tiles) that take
 // every part, but none that a batch of max_len cannot fill

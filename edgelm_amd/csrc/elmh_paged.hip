@@ -840,6 +840,9 @@ struct PagedRegs {
   f32x4 ks[COLS ? 2 : 1], vs[COLS ? 2 : 1];
 };
 
+// Registers for two workgroups a CU, or one (part_workgroups; also the q4 columns of 256, which fit: 38 us, 41 with one).
+constexpr int attention_fits(int dt, int NB, bool cols) { return part_workgroups(dt, 32 * NB) > 256 || cols ? 2 : 1; }
+
 // One workgroup: one part of one sequence's cache for up to 16 query heads of one kv head, its waves taking 32 tokens at a time.
 // Scores as K Q^T (tokens x heads) leave a lane with four tokens of one head, which is what the second product V^T P^T takes
 // as its operand: no exchange between lanes but the maximum over the four lane groups. One pass: running maximum m and sum l.
@@ -853,7 +856,7 @@ struct PagedRegs {
 // then added over them; and its weights take its own group's value scales, so that one split of 8 weights serves in place of
 // NB.
 template <int DT, int NB, bool COLS>
-__global__ __launch_bounds__(64 * kPaWaves, NB <= 4 ? 2 : 1) void paged_attention_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int HD = 32 * NB, OP = op_of(DT), PC = pieces_of(DT);
   extern __shared__ float lds[];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
