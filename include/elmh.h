@@ -301,7 +301,8 @@ int elmh_rope_dev(elmh_ctx* ctx, const float* x, float* y, int T, int n_heads, i
 /* Writes n tokens' keys (rotated first unless rope is NULL) and values into the cache: row i's head h at k + i * row + h *
  * head, strides in values (0: contiguous [n][n_kv][head_dim]), goes to position pos[i] of sequence seq[i] (i where seq is
  * NULL, and then n <= n_seqs). A row is skipped, and the cache left as it was, where its position is negative (padding), past
- * the table's pages or the rotary tables, its sequence is not one of n_seqs, or the table names no page. Finite values. */
+ * the table's pages or the rotary tables, its sequence is not one of n_seqs, or the table names no page. Values: finite
+ * in f32 and in the cache's type. The pools of keys and of values, and their scales, are different memory. */
 int elmh_paged_append_dev(elmh_ctx* ctx, const float* k, const float* v, int n, int64_t row, int64_t head,
                           const elmh_kv_pages* pages, const int32_t* table, int n_seqs, int max_pages, const int32_t* pos,
                           const int32_t* seq, const elmh_rope* rope);
@@ -315,7 +316,8 @@ int elmh_paged_read_dev(elmh_ctx* ctx, float* k, float* v, int n, int64_t row, i
  * rotated at position lens[s] - 1: the new token's key and value are in the cache already (elmh_paged_append_dev). out [n_seqs,
  * n_heads * head_dim], not overlapping q. lens is read on the device and bounded to 0 .. max_len; max_len, the host's bound,
  * sizes the launch. A sequence of length 0 (padding) gives zeros; positions of no page are left out; slots behind a sequence's
- * end may hold anything. Products and sums in f32 or as exact as it (quantized levels are multiplied as they are).
+ * end may hold anything. Products and sums in f32 or as exact as it (quantized levels are multiplied as they are); the values'
+ * sum is divided at its end, so a value times the number of positions has to be finite too.
  * At most 4096 sequences, 256 query heads a kv head, and n_seqs * max_len of 2^35.
  * Long sequences are split over workgroups and joined, in a device buffer the context allocates and grows outside capture
  * (elmh_scratch_generation); results do not depend on the order in which the parts end. */
