@@ -840,6 +840,8 @@ struct PagedRegs {
   f32x4 ks[COLS ? 2 : 1], vs[COLS ? 2 : 1];
 };
 
+// Heads whose groups of 32 values fit in the 16 columns of a tile
+constexpr int cols_heads(int NB) { return NB <= 2 ? 8 : NB <= 4 ? 4 : 2; }
 // Registers for two workgroups a CU, or one (part_workgroups; also the q4 columns of 256, which fit: 38 us, 41 with one).
 constexpr int attention_fits(int dt, int NB, bool cols) { return part_workgroups(dt, 32 * NB) > 256 || cols ? 2 : 1; }
 
@@ -851,7 +853,8 @@ constexpr int attention_fits(int dt, int NB, bool cols) { return part_workgroups
 // sequences of 8 to 16 thousand, 980 MB: 5.0 TB/s, vector ALUs 66% and matrix cores 23% busy), by the way to the first rows, four
 // dependent loads, where it is short (137 f32 positions: 6.6 us a call). Four waves: with eight the same cases took 87 us for 79
 // and 246 for 205. 32 tokens a step: the depth of a 16-bit matrix instruction in the second product.
-// COLS (q4, where the heads times the NB groups of 32 fit in the 16 columns): column n = h + j 16 / NB is head h and group j. Its
+// COLS (q4, where the heads times the NB groups of 32, made a power of two, fit in the 16 columns): column n = h + j HS, of the HS
+// heads that fit, is head h and group j. Its
 // query is zero outside the group, so a score's NB parts come out in NB lanes, each multiplied by its own group's scale and
 // then added over them; and its weights take its own group's value scales, so that one split of 8 weights serves in place of
 // NB.
@@ -887,8 +890,9 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
   const uint8_t* vpool = static_cast<const uint8_t*>(pg.v);
   const uint32_t koff = key_offset<DT, NB>(n, g), voff = 4 * g * RB;
   // the lane's scales: group j of block u, as PagedRegs says
-  constexpr int HS = COLS ? 16 / NB : 16;
-  const int sj = COLS ? n / HS : NG > 1 ? min(n / 2, NG - 1) : 0, su = n & 1;
+  constexpr int HS = COLS ? cols_heads(NB) : 16;
+  const int cj = n / HS;  // COLS: the column's group; past the last one its sums are 0 and not looked at
+  const int sj = COLS ? min(cj, NG - 1) : NG > 1 ? min(n / 2, NG - 1) : 0, su = n & 1;
   const uint32_t soff = (uint32_t)(sj * ps + 4 * g) * 4;
   const int qn = COLS ? n % HS : n;  // the lane's head
 
@@ -984,8 +988,8 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
       big = max_over_groups(big);
       if constexpr (COLS) {
         big = max_of(big, dpp_f<kDppRowRor8>(big));
-        if constexpr (NB >= 4) big = max_of(big, dpp_f<kDppRowRor4>(big));
-        if constexpr (NB >= 8) big = max_of(big, dpp_f<kDppRowRor2>(big));
+        if constexpr (HS <= 4) big = max_of(big, dpp_f<kDppRowRor4>(big));
+        if constexpr (HS <= 2) big = max_of(big, dpp_f<kDppRowRor2>(big));
       }
       const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255) - 127, -100), 127);
       const float up = pow2(9 - ex);
@@ -1002,7 +1006,7 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
       for (int p = 0; p < PC; ++p) {
         const u32x4 o = qo[0][p];
 #pragma unroll
-        for (int j = 0; j < NB; ++j) qo[j][p] = sj == j ? o : u32x4{0, 0, 0, 0};
+        for (int j = 0; j < NB; ++j) qo[j][p] = cj == j ? o : u32x4{0, 0, 0, 0};
       }
     }
   }
@@ -1044,8 +1048,8 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
         if constexpr (COLS) {  // the same sum in all of a head's lanes: halves, then quarters, ...
           v *= r.ks[u][i];
           v += dpp_f<kDppRowRor8>(v);
-          if constexpr (NB >= 4) v += dpp_f<kDppRowRor4>(v);
-          if constexpr (NB >= 8) v += dpp_f<kDppRowRor2>(v);
+          if constexpr (HS <= 4) v += dpp_f<kDppRowRor4>(v);
+          if constexpr (HS <= 2) v += dpp_f<kDppRowRor2>(v);
         } else if constexpr (DT == ELMH_Q8) {
           v *= row_bcast<u>(r.ks[0][i]);
         }
@@ -1167,7 +1171,7 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
   if (qn < heads) {
 #pragma unroll
     for (int x = 0; x < 2 * NB; ++x)
-      if (!COLS || x / 2 == sj) {
+      if (!COLS || x / 2 == cj) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) lds[(wave * heads + qn) * HD + value_dim<DT, NB>(x, 4 * g + i)] = acc[x][i];
       }
@@ -1290,8 +1294,8 @@ hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, int ext
 }
 template <int DT, int NB>
 hipError_t launch_paged_attention_cols(const PagedAttnArgs& a, int n_seqs, int extra, hipStream_t s) {
-  if constexpr (DT == ELMH_Q4 && (NB == 2 || NB == 4 || NB == 8))
-    if (a.group * NB <= kPaHeads) return launch_paged_attention_as<DT, NB, true>(a, n_seqs, extra, s);
+  if constexpr (DT == ELMH_Q4 && NB > 1)
+    if (a.group <= cols_heads(NB)) return launch_paged_attention_as<DT, NB, true>(a, n_seqs, extra, s);
   return launch_paged_attention_as<DT, NB, false>(a, n_seqs, extra, s);
 }
 template <int DT>

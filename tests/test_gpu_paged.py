@@ -252,6 +252,27 @@ def test_attention_of_wide_tiles(ctx, dtype, hd, grp):
     c.free()
 
 
+@pytest.mark.parametrize("hd", HDS)
+@pytest.mark.parametrize("grp", [1, 2, 3, 4, 5, 8, 9])
+def test_attention_of_q4_columns(ctx, hd, grp):
+    """Heads and groups of 32 values that share a tile's columns: as many as fit, fewer, one more; a row of the table without
+    pages, sequences in one part and in several."""
+    print(f"q4 columns hd {hd} group {grp}", flush=True)
+    rng = np.random.default_rng([hd, grp])
+    lens, page, n_kv = [700, 0, 37, 1, 60], 32, 2
+    table = _table_of(rng, lens, page, 30)
+    table[4, 0] = -1
+    c = Cache(ctx, "q4", n_kv, hd, page, 30)
+    _fill(c, rng, table, lens)
+    c.send()
+    q = rng.normal(0, 1, (5, n_kv * grp, hd)).astype(np.float32)
+    want, tol = _attention64(c, q, table, lens)
+    _check(_attend(ctx, c, q, table, lens), want, tol)
+    want, tol = _attention64(c, q, table, [500, 0, 37, 1, 60])
+    _check(_attend(ctx, c, q, table, [500, 0, 37, 1, 60], max_len=500), want, tol)
+    c.free()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "q8"])
 @pytest.mark.parametrize("rot,inter", [(128, False), (128, True), (64, False), (20, True), (22, False), (2, False)])
 def test_attention_rotates_queries(ctx, dtype, rot, inter):
