@@ -22,6 +22,11 @@ using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+// loads of words that lie on less than their size
+using u32_on1 = __attribute__((aligned(1))) uint32_t;
+using u32_on2 = __attribute__((aligned(2))) uint32_t;
+using u32x3_on4 = __attribute__((ext_vector_type(3), aligned(4))) uint32_t;
+using u32x4_on8 = __attribute__((ext_vector_type(4), aligned(8))) uint32_t;
 
 // ---------------------------------------------------------------- rotary tables and rotation
 
@@ -663,12 +668,15 @@ __device__ __forceinline__ void load_key(const uint8_t* base, uint32_t off, int 
     for (int j = 0; j + 1 < NB; j += 2) load_words<4>(base + (off + 16 * g) + 32 * j, w + 2 * j);
     if constexpr (NB % 2) load_words<2>(base + (off + 8 * g) + 32 * (NB - 1), w + 2 * (NB - 1));
   } else if constexpr (DT == ELMH_Q4) {
-    if constexpr (NB == 3) {  // 12 g: not on 8 bytes
+    if constexpr (NB == 3) {  // at 12 g
+      const u32x3_on4 v = *reinterpret_cast<const u32x3_on4*>(base + off);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) w[j] = *reinterpret_cast<const uint32_t*>(base + off + 4 * j);
-    } else if constexpr (NB == 6) {  // 24 g: on 8
+      for (int j = 0; j < 3; ++j) w[j] = v[j];
+    } else if constexpr (NB == 6) {  // at 24 g
+      const u32x4_on8 v = *reinterpret_cast<const u32x4_on8*>(base + off);
 #pragma unroll
-      for (int j = 0; j < NB; j += 2) load_words<2>(base + off + 4 * j, w + j);
+      for (int j = 0; j < 4; ++j) w[j] = v[j];
+      load_words<2>(base + off + 16, w + 4);
     } else {
       load_words<NB>(base + off, w);
     }
@@ -698,6 +706,7 @@ __device__ __forceinline__ u32x4 key_operand(const uint32_t (&w)[key_words(DT, N
 }
 
 // row: a token's value row less the lane's offset, off; n: the lane's part of it
+// (As few loads as there can be: with a q4 row of 96 read by bytes, 24 sequences of 8 to 16 thousand took 73 us, so 47.)
 template <int DT, int NB>
 __device__ __forceinline__ void load_value(const uint8_t* row, uint32_t off, int n, uint32_t (&w)[value_words(DT, NB)]) {
   if constexpr (DT == ELMH_Q4) {  // NB bytes at n * NB
@@ -706,12 +715,10 @@ __device__ __forceinline__ void load_value(const uint8_t* row, uint32_t off, int
     } else if constexpr (NB == 2) {
       w[0] = *reinterpret_cast<const uint16_t*>(row + (off + 2 * n));
     } else if constexpr (NB == 3) {
-      const uint8_t* p = row + (off + 3 * n);
-      w[0] = p[0] | p[1] << 8 | p[2] << 16;
+      w[0] = *reinterpret_cast<const u32_on1*>(row + (off + 3 * n - (n == 15)));  // the last lane's from its second byte on
     } else if constexpr (NB == 6) {
-      const uint16_t* p = reinterpret_cast<const uint16_t*>(row + (off + 6 * n));
-      w[0] = p[0] | (uint32_t)p[1] << 16;
-      w[1] = p[2];
+      w[0] = *reinterpret_cast<const u32_on2*>(row + (off + 6 * n));
+      w[1] = *reinterpret_cast<const uint16_t*>(row + (off + 6 * n + 4));
     } else {
       load_words<NB / 4>(row + (off + NB * n), w);
     }
@@ -733,7 +740,7 @@ __device__ __forceinline__ void load_value(const uint8_t* row, uint32_t off, int
 // The operand of value x over eight tokens: v[0..3] the first block's, v[4..7] the second's. q4: of an odd x the byte that holds it
 // and its neighbour, 16 times the one plus the other: the neighbour's sum is taken off at the end (after the last tile).
 template <int DT, int NB>
-__device__ __forceinline__ u32x4 value_operand(const uint32_t (&v)[8][value_words(DT, NB)], int x) {
+__device__ __forceinline__ u32x4 value_operand(const uint32_t (&v)[8][value_words(DT, NB)], int x, int n) {
   u32x4 o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -743,7 +750,7 @@ __device__ __forceinline__ u32x4 value_operand(const uint32_t (&v)[8][value_word
       o[i] = f16_bytes(__builtin_amdgcn_perm(b, a, sel));  // the bytes were flipped to q + 128
     } else if constexpr (DT == ELMH_Q4) {
       const int j = x / 2;
-      const uint32_t sel = 0x0C040C00u + (j % 4) * 0x00010001u;
+      const uint32_t sel = 0x0C040C00u + (j % 4 + (NB == 3 && n == 15)) * 0x00010001u;
       const uint32_t w = __builtin_amdgcn_perm(v[2 * i + 1][j / 4], v[2 * i][j / 4], sel);
       o[i] = x % 2 ? f16_nibble_bytes(w) : f16_low_nibbles(w);
     } else {
@@ -1144,7 +1151,7 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
         split8<OP>(t, po, minus_one);
 #pragma unroll
         for (int x = j * 2 * NB / runs; x < (j + 1) * 2 * NB / runs; ++x) {
-          const u32x4 vo = value_operand<DT, NB>(r.v, x);
+          const u32x4 vo = value_operand<DT, NB>(r.v, x, n);
 #pragma unroll
           for (int k = PC - 1; k >= 0; --k) acc[x] = mfma<OP>(vo, po[k], acc[x]);
         }
