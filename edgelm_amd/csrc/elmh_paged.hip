@@ -847,10 +847,8 @@ struct PagedRegs {
   f32x4 ks[COLS ? 2 : 1], vs[COLS ? 2 : 1];
 };
 
-// Heads whose groups of 32 values fit in the 16 columns of a tile
-constexpr int cols_heads(int NB) { return NB <= 2 ? 8 : NB <= 4 ? 4 : 2; }
-// Registers for two workgroups a CU, or one (part_workgroups; also the q4 columns of 256, which fit: 38 us, 41 with one).
-constexpr int attention_fits(int dt, int NB, bool cols) { return part_workgroups(dt, 32 * NB) > 256 || cols ? 2 : 1; }
+// Registers for two workgroups a CU, or one
+constexpr int attention_fits(int dt, int NB, bool cols) { return part_workgroups(dt, 32 * NB, cols) > 256 ? 2 : 1; }
 
 // One workgroup: one part of one sequence's cache for up to 16 query heads of one kv head, its waves taking 32 tokens at a time.
 // Scores as K Q^T (tokens x heads) leave a lane with four tokens of one head, which is what the second product V^T P^T takes
@@ -897,7 +895,7 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
   const uint8_t* vpool = static_cast<const uint8_t*>(pg.v);
   const uint32_t koff = key_offset<DT, NB>(n, g), voff = 4 * g * RB;
   // the lane's scales: group j of block u, as PagedRegs says
-  constexpr int HS = COLS ? cols_heads(NB) : 16;
+  constexpr int HS = COLS ? cols_heads(HD) : 16;
   const int cj = n / HS;  // COLS: the column's group; past the last one its sums are 0 and not looked at
   const int sj = COLS ? min(cj, NG - 1) : NG > 1 ? min(n / 2, NG - 1) : 0, su = n & 1;
   const uint32_t soff = (uint32_t)(sj * ps + 4 * g) * 4;
@@ -1302,7 +1300,7 @@ hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, int ext
 template <int DT, int NB>
 hipError_t launch_paged_attention_cols(const PagedAttnArgs& a, int n_seqs, int extra, hipStream_t s) {
   if constexpr (DT == ELMH_Q4 && NB > 1)
-    if (a.group <= cols_heads(NB)) return launch_paged_attention_as<DT, NB, true>(a, n_seqs, extra, s);
+    if (part_cols(DT, 32 * NB, a.group)) return launch_paged_attention_as<DT, NB, true>(a, n_seqs, extra, s);
   return launch_paged_attention_as<DT, NB, false>(a, n_seqs, extra, s);
 }
 template <int DT>
@@ -1443,7 +1441,7 @@ hipError_t launch_paged_read(float* k, float* v, int n, int64_t row, int64_t hea
 
 PagedSplit paged_attention_split(int dtype, int n_seqs, int n_heads, int n_kv, int head_dim, int max_len) {
   const int rows = n_kv * ((n_heads / n_kv + kPaHeads - 1) / kPaHeads);
-  const int workgroups = part_workgroups(dtype, head_dim);
+  const int workgroups = part_workgroups(dtype, head_dim, part_cols(dtype, head_dim, n_heads / n_kv));
   PagedSplit p;
   p.extra = part_extra(workgroups, rows, n_seqs, max_len);
   p.rule = part_rule(workgroups, rows, n_seqs, max_len, p.extra);
