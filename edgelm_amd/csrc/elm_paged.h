@@ -66,7 +66,16 @@ ELM_HD int64_t kv_page_of(const int32_t* table_row, int max_pages, int64_t n_pag
 constexpr int kPartLeastUnits = 4;   // of a part: one unit a wave
 constexpr int kPartAloneUnits = 16;  // sequences up to this are not split: the second launch costs more (q8, 200 positions: 8.5 us
                                      // in one, 11.6 split; 500: 10.7 and 11.5; 1000: 14.4 and 11.5)
-inline int part_least(int max_len) { return max_len <= kPartAloneUnits * kSplitUnit ? kPartAloneUnits : kPartLeastUnits; }
+// Where the whole batch is a few workgroups and a unit takes long (large heads, f32), fewer: 2048 / head_dim, for f32 half of that
+// (4 kv heads, 8 sequences of up to 500: f32 of 128 13.0 us, unsplit 18.4; f32 of 256 23.6 and 42; q4 of 256 13.6 and 17.8; of up
+// to 300, split all the same, q8 of 192 14.0, unsplit 12.7. At 128 workgroups f32 of 128 takes 21.7 us split, 19.8 unsplit.)
+constexpr int kPartFewWorkgroups = 64;
+inline int part_alone(int dtype, int head_dim, int workgroups) {
+  if (workgroups > kPartFewWorkgroups) return kPartAloneUnits;
+  const int units = 2048 / (dtype == ELMH_F32 ? 2 * head_dim : head_dim);
+  return units < kPartAloneUnits ? units : kPartAloneUnits;
+}
+inline int part_least(int max_len, int alone) { return max_len <= alone * kSplitUnit ? alone : kPartLeastUnits; }
 constexpr int kPartFairUnits = 12;   // a part that is worth its start and end
 constexpr int kPartLongUnits = 64;   // a part whose start and end no longer matter
 constexpr int kPartMostExtra = 1024;
@@ -125,8 +134,8 @@ struct PartRule {
   CeilDiv few, once, extra;
   int least = 1;
 };
-inline PartRule part_rule(int workgroups, int rows, int n_seqs, int max_len, int extra) {
-  return {ceil_div(part_few(rows, extra)), ceil_div(part_once(workgroups, rows, n_seqs, extra)), ceil_div(extra), part_least(max_len)};
+inline PartRule part_rule(int workgroups, int rows, int n_seqs, int max_len, int extra, int alone = kPartAloneUnits) {
+  return {ceil_div(part_few(rows, extra)), ceil_div(part_once(workgroups, rows, n_seqs, extra)), ceil_div(extra), part_least(max_len, alone)};
 }
 // Units a part: the batch's `total` over `once`, but of kPartFairUnits as long as `few` parts (one workgroup a CU) are left; where
 // that gives parts of kPartLongUnits and more, over up to `extra`, so that uneven ends even out. (64 q4 sequences of 8 to 16

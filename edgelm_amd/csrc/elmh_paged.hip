@@ -1444,7 +1444,7 @@ PagedSplit paged_attention_split(int dtype, int n_seqs, int n_heads, int n_kv, i
   const int workgroups = part_workgroups(dtype, head_dim, part_cols(dtype, head_dim, n_heads / n_kv));
   PagedSplit p;
   p.extra = part_extra(workgroups, rows, n_seqs, max_len);
-  p.rule = part_rule(workgroups, rows, n_seqs, max_len, p.extra);
+  p.rule = part_rule(workgroups, rows, n_seqs, max_len, p.extra, part_alone(dtype, head_dim, n_seqs * rows));
   if (max_len > p.rule.least * kSplitUnit)
     p.part_bytes = ((size_t)n_seqs + p.extra) * n_heads * (head_dim + 2) * sizeof(float) + n_seqs * sizeof(int2);
   return p;

@@ -33,6 +33,7 @@ int rope(const float* x, const float* y, int64_t T, int nh, int hd, int64_t xr, 
 int table(const float* c, const float* s, int64_t p0, int64_t n, int rot, double th, const elmh_rope_scaling* sc) {
   return code(check_rope_table(c, s, p0, n, rot, th, sc));
 }
+int alone(int dt, int hd, int workgroups) { return part_alone(dt, hd, workgroups); }
 int64_t page_of(const int32_t* row, int mp, int64_t np, int pos, int ps) { return kv_page_of(row, mp, np, pos, page_magic(ps)); }
 int page_index_of(int pos, int ps) { return page_index(pos, page_magic(ps)); }
 int extra(int dt, int hd, int rows, int n, int max_len) { return part_extra(part_workgroups(dt, hd), rows, n, max_len); }
@@ -278,3 +279,14 @@ def test_scaled_frequencies(host):
             for kind, w in want.items():
                 sc = None if kind is None else E.RopeScaling(kind, fac, orig, lo, hi if kind == E.ROPE_BANDS else 32.0)
                 assert abs(host.freq(rot, th, sc, i) / w - 1) <= 64 * 2.0 ** -53, (kind, rot, i)
+
+
+def test_short_sequences_stay_whole(host):
+    """The longest sequence that is not split, in units of 32 positions: sixteen, fewer where a unit takes long and the batch is
+    few workgroups, never under a part's least."""
+    for dt in (E.F32, E.F16, E.BF16, E.Q8, E.Q4):
+        for hd in (32, 64, 96, 128, 192, 256):
+            assert host.alone(dt, hd, 65) == 16
+            for workgroups in (1, 64):
+                assert host.alone(dt, hd, workgroups) == min(16, 2048 // (hd * (2 if dt == E.F32 else 1)))
+                assert 4 <= host.alone(dt, hd, workgroups) <= 16
