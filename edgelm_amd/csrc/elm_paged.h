@@ -85,13 +85,12 @@ constexpr bool part_cols(int dtype, int head_dim, int group) {
   return dtype == ELMH_Q4 && head_dim > 32 && group <= cols_heads(head_dim);
 }
 // Workgroups that are on the card together: as many a CU as the kernel's registers leave room for, one to four. Above a head size
-// of 128 two fit where the cache has few bytes (256 registers a lane without spilling: a 16-bit type to 192, q8, q4 to 192 or in
-// columns), and are worth up to a sixth (8 sequences of 4 to 8 thousand, 4 kv heads: q4 of 192 24.2 us, with one 28.8; q8 of 256
-// 36 and 37). Counting three where two fit (q4 of 128, more heads than columns) costs up to a fifth: 54 sequences of up to 6000
-// 53 us, so 48; 3 of up to 36 thousand 27 and 22. (bf16 of 96 fits three, and is better counted as two: 16 sequences of up to
-// 3000 19 us, as three 20; two of some 70 thousand 96 and 92.)
+// of 128 two fit where the cache has few bytes (a 16-bit type to 192, q8, q4), and are worth up to a sixth (8 sequences of 4 to 8
+// thousand, 4 kv heads: q4 of 192 24.2 us, with one 28.8; q8 of 256 36 and 37). Counting three where two fit (q4 of 128, more heads
+// than columns) costs up to a fifth: 54 sequences of up to 6000 53 us, so 48; 3 of up to 36 thousand 27 and 22. (bf16 of 96 fits
+// three, and is better counted as two: 16 sequences of up to 3000 19 us, as three 20; two of some 70 thousand 96 and 92.)
 constexpr int part_workgroups(int dtype, int head_dim, bool cols = false) {
-  if (head_dim > 128) return 256 * (dtype == ELMH_Q8 || cols || (dtype != ELMH_F32 && head_dim <= 192) ? 2 : 1);
+  if (head_dim > 128) return 256 * (dtype == ELMH_Q8 || dtype == ELMH_Q4 || (dtype != ELMH_F32 && head_dim <= 192) ? 2 : 1);
   const bool two = dtype == ELMH_F32 || dtype == ELMH_BF16 || (dtype == ELMH_Q4 && head_dim > 96 && !cols);
   return 256 * (head_dim <= 64 ? 4 : two ? 2 : 3);
 }

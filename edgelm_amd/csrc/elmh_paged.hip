@@ -849,6 +849,9 @@ struct PagedRegs {
 
 // Registers for two workgroups a CU, or one
 constexpr int attention_fits(int dt, int NB, bool cols) { return part_workgroups(dt, 32 * NB, cols) > 256 ? 2 : 1; }
+// Query operands that stay in LDS (the same for all waves; [group][piece][lane] of 16 bytes): 64 registers less, so that two
+// workgroups fit a CU (8 sequences of 17591 with 7 queries a kv head: 71 us, 108 with one; at 128 and 192 it gains nothing).
+constexpr bool query_in_lds(int dt, int NB, bool cols) { return dt == ELMH_Q4 && NB == 8 && !cols; }
 
 // One workgroup: one part of one sequence's cache for up to 16 query heads of one kv head, its waves taking 32 tokens at a time.
 // Scores as K Q^T (tokens x heads) leave a lane with four tokens of one head, which is what the second product V^T P^T takes
@@ -1016,6 +1019,19 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
     }
   }
 
+  constexpr bool QLDS = query_in_lds(DT, NB, COLS);
+  const u32x4* qlds = reinterpret_cast<const u32x4*>(lds) + lane;
+  if constexpr (QLDS) {
+    lds_barrier();  // the queries have been read
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (j % kPaWaves == wave) {
+#pragma unroll
+        for (int p = 0; p < PC; ++p) reinterpret_cast<u32x4*>(lds)[64 * (PC * j + p) + lane] = qo[j][p];
+      }
+    lds_barrier();
+  }
+
   float m = -INFINITY, l = 0.f;
   int vexp = -100;  // q8, q4: the softmax weights take the value scales over 2^vexp, the largest seen
   f32x4 acc[2 * NB];
@@ -1025,6 +1041,8 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
   const auto step = [&](auto more) {
     const bool whole = tile.valid[0] == kPageStep && tile.valid[1] == kPageStep;
     float s[8];
+    int qat = 0;
+    if constexpr (QLDS) asm("" : "+v"(qat));  // read in each step: the compiler would keep them in registers again
     static_for<2>([&](auto U) {
       constexpr int u = U;
       f32x4 sc{0.f, 0.f, 0.f, 0.f};
@@ -1038,7 +1056,7 @@ __global__ __launch_bounds__(64 * kPaWaves, attention_fits(DT, NB, COLS)) void p
           constexpr bool apart = DT == ELMH_Q4 && !COLS;  // groups' sums, each with its scale
           f32x4 t = apart ? f32x4{0.f, 0.f, 0.f, 0.f} : sc;
 #pragma unroll
-          for (int p = PC - 1; p >= 0; --p) t = mfma<OP>(ko, qo[j][p], t);
+          for (int p = PC - 1; p >= 0; --p) t = mfma<OP>(ko, QLDS ? qlds[qat + 64 * (PC * j + p)] : qo[j][p], t);
           if constexpr (apart) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) sc[i] = fmaf(row_bcast<2 * j + u>(r.ks[0][i]), t[i], sc[i]);
@@ -1285,7 +1303,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedAttnArgs 
 template <int DT, int NB, bool COLS>
 hipError_t launch_paged_attention_as(const PagedAttnArgs& a, int n_seqs, int extra, hipStream_t s) {
   const int heads = a.group < kPaHeads ? a.group : kPaHeads;
-  const size_t lds = (size_t)(kPaWaves * heads * 32 * NB + 2 * kPaWaves * kPaHeads + kPaWaves) * sizeof(float);
+  size_t lds = (size_t)(kPaWaves * heads * 32 * NB + 2 * kPaWaves * kPaHeads + kPaWaves) * sizeof(float);
+  if constexpr (query_in_lds(DT, NB, COLS)) lds = std::max<size_t>(lds, NB * pieces_of(DT) * 64 * sizeof(u32x4));
   if (lds > 64 * 1024) {
     static DeviceOnce once;
     if (!raise_dynamic_lds(once, (const void*)paged_attention_kernel<DT, NB, COLS>, 80 * 1024)) return hipErrorInvalidValue;
